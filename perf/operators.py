@@ -277,17 +277,12 @@ _PLAIN = dict(route=_plain_route, sort=_plain_sort, merge=_plain_merge, merge_gr
 
 
 # ---------------------------------------------------------------------------------------------- one pass
-_package = None
-
-
 def _bz():
-    """the package, imported by the first pass, as a user's program imports it once"""
-    global _package
-    if _package is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "x-deeplearning_amd"))
-        import blaze_hip
-        _package = blaze_hip
-    return _package
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "x-deeplearning_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import blaze_hip
+    return blaze_hip
 
 
 def _own_route(bz, st):
