@@ -973,3 +973,58 @@ int main() {
                     "-I" + os.path.join(ROOT, "x-deeplearning_amd", "csrc"), str(src), "-o", exe], check=True, capture_output=True, timeout=300)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stdout[-2000:], r.stderr[-3000:])
+
+
+def test_a_thread_that_ends_waits_for_its_streams(tmp_path):
+    """An event recorded on a stream is worth nothing once the stream has been destroyed with commands in flight: before a thread's stream
+    goes, it is waited for, whatever the thread queued there (a HIP runtime of counters stands in for the real one)."""
+    import shutil
+    import subprocess
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    csrc = os.path.join(ROOT, "x-deeplearning_amd", "csrc")
+    src, exe = tmp_path / "streams.cc", str(tmp_path / "streams")
+    src.write_text(r"""
+#include <stdio.h>
+#include <map>
+#include <thread>
+#include "blaze/runtime.h"
+namespace {
+int made = 0, destroyed = 0, late = 0;
+std::map<hipStream_t, int> queued;  // commands that nobody has waited for
+}
+extern "C" {
+hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) { *s = (hipStream_t)(uintptr_t)(0x1000 * ++made); queued[*s] = 0; return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t s) { queued[s] = 0; return hipSuccess; }
+hipError_t hipStreamDestroy(hipStream_t s) { ++destroyed; late += queued[s] != 0; return hipSuccess; }
+hipError_t hipMemcpyAsync(void*, const void*, size_t, hipMemcpyKind, hipStream_t s) { ++queued[s]; return hipSuccess; }
+hipError_t hipGetDevice(int* d) { *d = 0; return hipSuccess; }
+hipError_t hipSetDevice(int) { return hipSuccess; }
+hipError_t hipMalloc(void**, size_t) { return hipErrorUnknown; }
+hipError_t hipFree(void*) { return hipSuccess; }
+hipError_t hipHostMalloc(void**, size_t, unsigned) { return hipErrorUnknown; }
+hipError_t hipHostFree(void*) { return hipSuccess; }
+hipError_t hipGetLastError(void) { return hipSuccess; }
+const char* hipGetErrorString(hipError_t) { return ""; }
+}
+int main() {
+  for (int device : {0, 2})
+    std::thread([&] {
+      blaze::DeviceOption option;
+      option.set_device_type(blaze::kHIP);
+      option.set_device_id(device);
+      for (int id = 0; id < 2; ++id) {
+        blaze::HIPContext context(option);
+        context.SwitchToDevice(id);
+        (void)hipMemcpyAsync(nullptr, nullptr, 4, hipMemcpyHostToDevice, context.hip_stream());
+      }
+    }).join();
+  printf("%d made, %d destroyed, %d with commands in flight\n", made, destroyed, late);
+  return made == 4 && destroyed == 4 && late == 0 ? 0 : 1;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(ROOT, "include"), "-I" + csrc, str(src),
+                    os.path.join(csrc, "blaze", "runtime.cc"), os.path.join(csrc, "blaze", "proto.cc"), os.path.join(csrc, "blaze", "common.cc"), "-o", exe],
+                   check=True, capture_output=True, timeout=300)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout

@@ -1742,3 +1742,31 @@ def test_few_rows_do_not_reach_into_each_other(pb, k):
     assert np.isnan(got[1][2]).all()
     for i, c, sign in ((0, 0, 1), (200, k - 1, -1), (389, k - 1, 1)):  # Sigmoid(e^x / (1 + e^x)) of +inf is NaN, of -inf 0: NaN where any output is +inf
         assert np.isnan(got[1][i]).all() == (sign * ws[0][c] > 0).any(), i
+
+
+@pytest.mark.parametrize("many", [True, False])
+def test_inputs_fed_by_threads_that_have_ended(pb, many):
+    """A request of several parts fed by a thread that ends while they are on their way: the pass on this thread's stream sees all of it."""
+    import threading
+    nb = pb.NetBuilder("ended", device_type=1)
+    nb.external_input("x", pb.K_FLOAT)
+    rng = np.random.default_rng(3)
+    w = rng.standard_normal((256, 4)).astype(np.float32)
+    nb.constant("w", w)
+    nb.op("Gemm", ["x", "w"], ["y"])
+    nb.external_output("y", pb.K_FLOAT)
+    pm = pb.PredictorManager()
+    pm.load_model_from_string(nb.text(), True)
+    p = pm.create_predictor(1, 0)
+    xs = [rng.standard_normal((5000, 256)).astype(np.float32) for _ in range(3)]
+    wants = [x.astype(np.float64) @ w for x in xs]
+    p.reshape_input("x", xs[0].shape)
+    for step in range(12):
+        x = xs[step % 3]
+        batch = p.feed_batch([("x", x)])
+        t = threading.Thread(target=(lambda: p.feed_many(batch)) if many else (lambda: p.feed("x", x)))
+        t.start()
+        t.join()
+        p.forward()
+        # sums of 256 products of numbers below 6
+        np.testing.assert_allclose(p.output_asnumpy("y"), wants[step % 3], rtol=0, atol=260 * 36 * 2.0**-24 * 256, err_msg="step %d" % step)

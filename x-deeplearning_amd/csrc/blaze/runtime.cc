@@ -88,10 +88,16 @@ struct ThreadStream {
 };
 struct ThreadStreams {
   std::vector<std::vector<ThreadStream>> per_device;
+  // What the thread has queued ends before its streams go: a stream that is destroyed may leave with commands in flight, and an event
+  // recorded on it then no longer stands for them.  (Seen once: a thread fed 300 x 64 floats and ended, and the pass on another thread's
+  // stream, behind that event, read 92 rows as they had been before, what six of the transfer's nineteen workgroups bring.)
   ~ThreadStreams() {
     for (auto& v : per_device)
       for (auto& s : v)
-        if (s.stream) (void)hipStreamDestroy(s.stream);
+        if (s.stream) {
+          (void)hipStreamSynchronize(s.stream);
+          (void)hipStreamDestroy(s.stream);
+        }
   }
   ThreadStream& at(int device_id, int stream_id) {
     BLAZE_CONDITION_THROW(device_id >= 0 && stream_id >= 0 && stream_id < kMaxStreamNum, "device_id=", device_id, " stream_id=", stream_id);
