@@ -1770,3 +1770,32 @@ def test_inputs_fed_by_threads_that_have_ended(pb, many):
         p.forward()
         # sums of 256 products of numbers below 6
         np.testing.assert_allclose(p.output_asnumpy("y"), wants[step % 3], rtol=0, atol=260 * 36 * 2.0**-24 * 256, err_msg="step %d" % step)
+
+
+def test_inputs_fed_one_by_one_from_several_threads(pb):
+    """Each input fed by a thread of its own that lives on, a long transfer before a short one and the other way round: the pass sees both."""
+    from concurrent.futures import ThreadPoolExecutor
+    nb = pb.NetBuilder("two", device_type=1)
+    for name in ("a", "b"):
+        nb.external_input(name, pb.K_FLOAT)
+    nb.constant("one", np.ones((1, 1), np.float32))
+    nb.op("Add", ["a", "one"], ["c"])
+    nb.op("Add", ["b", "one"], ["d"])
+    for name in ("c", "d"):
+        nb.external_output(name, pb.K_FLOAT)
+    pm = pb.PredictorManager()
+    pm.load_model_from_string(nb.text(), True)
+    p = pm.create_predictor(1, 0)
+    shapes = {"a": (20000, 512), "b": (3, 2)}
+    for name, shape in shapes.items():
+        p.reshape_input(name, shape)
+    threads = {name: ThreadPoolExecutor(1) for name in shapes}
+    for step in range(8):
+        value = {"a": np.float32(step), "b": np.float32(-step)}
+        for name in ("a", "b") if step % 2 == 0 else ("b", "a"):
+            threads[name].submit(p.feed, name, np.full(shapes[name], value[name], np.float32)).result()
+        p.forward()
+        for name, out in (("a", "c"), ("b", "d")):
+            assert (p.output_asnumpy(out) == value[name] + 1).all(), (step, name)
+    for t in threads.values():
+        t.shutdown()

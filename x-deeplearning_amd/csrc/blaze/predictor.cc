@@ -154,9 +154,10 @@ bool Predictor::Feed(size_t idx, const void* data, size_t len) {
         blob->Reshape(shape);
       }
       SettleBefore(ctx);
-      // stage in pinned memory and queue the transfer; a second Feed of the same input first waits for the first
+      // stage in pinned memory and queue the transfer; a second Feed of the same input first waits for the first, and one from another
+      // thread for all before it: the event and the pass stand behind one stream's transfers
       if (feed_done_ == nullptr) HIP_CHECK(hipEventCreateWithFlags(&feed_done_, hipEventDisableTiming));
-      if (feed_pending_[idx]) FinishFeeds();
+      if (feed_pending_[idx] || (any_feed_pending_ && feed_on_ != ctx.stream_serial())) FinishFeeds();
       Blob* stage = input_cpu_[idx].get();
       stage->set_data_type((DataType)blob->data_type());
       stage->Reshape(blob->shape());
