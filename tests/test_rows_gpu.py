@@ -825,3 +825,30 @@ def test_tensors_that_do_not_fit_are_refused(bz):
     with pytest.raises(bz.BlazeHipError, match="act_params"):
         bz.grouped_fc(_normal(0, (4, 8)), _normal(1, (2, 6, 8)), torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda"), 8, act=bz.ACT_PRELU,
                       act_params=(_normal(2, (2, 5)), ))
+
+
+# ---------------------------------------------------------------------------------------------- rows of zeros
+# (rows, columns, K, groups, elements between rows of w beyond K): the kernel for few rows, both kinds of the one for rows that begin anywhere, the one for
+# many rows
+ZERO_ROWS = [(40, 24, 64, 3, 0), (4096, 1024, 64, 8, 0), (3000, 700, 72, 3, 1), (2500, 1000, 45, 2, 0)]
+
+
+@pytest.mark.parametrize("m,n,k,groups,pad", ZERO_ROWS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "sigmoid", "swiglu"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_grouped_fc_of_no_rows_at_all(bz, m, n, k, groups, pad, dtype, act, bias):
+    """an `a` of no rows: every row number is outside, and every row is one of zeros"""
+    import torch
+    print("case", m, n, k, groups, pad, dtype, act, bias, flush=True)
+    cols = 2 * n if act == "swiglu" else n
+    w = _pitched(_normal(1, (groups, cols, k), 1.0, dtype), pad, float("nan"))
+    b = _normal(2, (groups, cols)) if bias else None
+    cuts = torch.tensor([m * g // groups for g in range(groups + 1)], dtype=torch.int32, device="cuda")
+    rows = torch.arange(m, dtype=torch.int32, device="cuda")
+    code = {"none": bz.ACT_NONE, "sigmoid": bz.ACT_SIGMOID, "swiglu": bz.ACT_SWIGLU}[act]
+    y = bz.grouped_fc(torch.empty((0, k), dtype=w.dtype, device="cuda"), w, cuts, k, rows=rows, rows_per=2, bias=b, act=code)
+    v = b.double() if bias else torch.zeros((groups, cols), dtype=torch.float64, device="cuda")
+    f = {"none": lambda v: v, "sigmoid": torch.sigmoid, "swiglu": lambda v: v[:, :n] * torch.sigmoid(v[:, :n]) * v[:, n:]}[act]
+    want = f(v).repeat_interleave(cuts[1:].long() - cuts[:-1].long(), 0)
+    _close(y, want, (HALF_STEP[dtype] + 32 * EPS) * want.abs() + (2.0**-25 if dtype == "f16" else 0.0), "y")

@@ -281,7 +281,7 @@ struct Column {
 // A workgroup of four waves owns BM rows of one group and BN columns (with GATED: BN / 2 columns, each with its gate's); a wave BM / 2 x
 // BN / 2 of them in 32x32 blocks.  K goes by in steps of 128 bytes a row, from global memory through registers into one of two LDS
 // buffers, the next step's loads in flight while this one is multiplied.  Chunk c of row r lies at position c ^ (r & 7).
-// It takes what the wide kernel cannot: rows that begin anywhere, operands beyond 4 GB.  Bound by the loads at odd addresses, two requests
+// It takes what the wide kernel cannot: rows that begin anywhere, operands beyond 4 GB, an `a` without rows.  Bound by the loads at odd addresses, two requests
 // where one would do: 2000 rows of 1023 -> 1023 bf16 23.1 us, 182 TFLOP/s (1024 -> 1024 by this kernel 20.0, by
 // the wide one 13.0).
 template <int DT, int BM, int BN, bool GATED, bool ADAPTERS>
@@ -805,7 +805,7 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
   const int lrow = wave * 8 + (lane >> 3), chunk = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7);
   auto a_off = [&](int r) {
     const char* row = input_row(l, min(m0 + r, m1 - 1), ES);
-    return row != nullptr ? (uint32_t)(row - l.a) : 0u;  // (a row of zeros: any other, whose sums are passed over)
+    return row != nullptr ? (uint32_t)(row - l.a) : 0u;  // (a row of zeros: the first one, whose sums are passed over)
   };
   auto w_off = [&](int r) {  // GATED: 32 columns and their 32 gates in turn
     const int col = GATED ? min(n0 + r / 64 * 32 + r % 32, l.n - 1) + (r / 32 % 2 ? l.n : 0) : min(n0 + r, l.n - 1);
@@ -1271,7 +1271,8 @@ int run_layer(const Layer& l, hipStream_t st) {
   const int groups = l.offsets ? l.groups : 1;
   const bool aligned = rows_aligned(l, In<DT>::kSize);
   const int64_t limit = (int64_t)1 << 32, es = In<DT>::kSize;
-  const bool near = l.a_count * l.lda * es <= limit && (int64_t)l.n * (GATED ? 2 : 1) * l.ldw * es <= limit;
+  // (the wide kernel reads some row where a row of zeros is asked for, so there has to be one)
+  const bool near = l.a_count > 0 && l.a_count * l.lda * es <= limit && (int64_t)l.n * (GATED ? 2 : 1) * l.ldw * es <= limit;
   auto tiles = [&](int rows, int cols) { return about_tiles(l.m, groups, rows) * ((l.n + cols - 1) / cols); };
   constexpr int G = GATED ? 2 : 1;
   const int64_t small = tiles(32, 32 / G);
