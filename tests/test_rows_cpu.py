@@ -116,3 +116,28 @@ def test_fc_adapters_refusals(bz):
     assert _rc(bz, "bz_fc_adapters", _fill(bz.FcAdaptersDesc, **dict(good, m=0, a=None)))[0] == bz.OK
     size = bz.lib().bz_fc_adapters_scratch_bytes
     assert size(32, 8) == 32 * 16 * 4 and size(1, 256) == 1024 and size(0, 8) == 0 and size(3, 17) == 3 * 32 * 4
+
+
+@pytest.mark.parametrize("act_size", [1, 23, 25, -1])
+def test_dice_of_one_parameter_a_group_is_refused(bz, act_size):
+    """Dice has a parameter a column: with fewer, the kernels would read behind them"""
+    dice = dict(act=bz.ACT_DICE, act_p0=P, act_p1=P, act_p2=P, n=24, k=16, in_dtype=bz.F16, out_dtype=bz.F16, lda=16, ldw=16, ldy=24)
+    for entry, desc, more in (("bz_grouped_fc", bz.GroupedFcDesc, dict(groups=4, w_stride=16 * 24)), ("bz_fc_adapters", bz.FcAdaptersDesc, {})):
+        rc, text = _rc(bz, entry, _fill(desc, **dict(dice, **more), act_size=act_size))
+        assert rc == bz.EINVAL and entry in text and "Dice" in text
+        for whole in (0, 24):
+            assert _rc(bz, entry, _fill(desc, **dict(dice, **more), act_size=whole))[0] == bz.OK
+
+
+def test_the_binding_refuses_dice_of_one_parameter_a_group(bz):
+    import torch
+    bz._here()  # (what the calls begin with)
+    for groups in (1, 3):
+        full, one = torch.zeros((groups, 8)), torch.zeros((groups, 1))
+        for params in ((one, full, full), (full, one, full), (full, full, one), (one, one, one)):
+            with pytest.raises(bz.BlazeHipError, match="act_params.* has %d elements" % groups):
+                bz._act_fields("grouped_fc", bz.ACT_DICE, params, 8, groups, -1)
+        assert bz._act_fields("grouped_fc", bz.ACT_DICE, (full, full, full), 8, groups, -1)[1] == 8
+        assert bz._act_fields("grouped_fc", bz.ACT_PRELU, (one, ), 8, groups, -1)[1] == 1
+        with pytest.raises(bz.BlazeHipError, match="act_params"):
+            bz._act_fields("grouped_fc", bz.ACT_PRELU, (full, one), 8, groups, -1)

@@ -852,3 +852,15 @@ def test_grouped_fc_of_no_rows_at_all(bz, m, n, k, groups, pad, dtype, act, bias
     f = {"none": lambda v: v, "sigmoid": torch.sigmoid, "swiglu": lambda v: v[:, :n] * torch.sigmoid(v[:, :n]) * v[:, n:]}[act]
     want = f(v).repeat_interleave(cuts[1:].long() - cuts[:-1].long(), 0)
     _close(y, want, (HALF_STEP[dtype] + 32 * EPS) * want.abs() + (2.0**-25 if dtype == "f16" else 0.0), "y")
+
+
+def test_dice_of_one_parameter_a_group_is_refused(bz):
+    """where a parameter a column is read"""
+    import torch
+    a, w, cuts = _normal(0, (4, 8)), _normal(1, (2, 6, 8)), torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    one, full = torch.ones((2, 1), device="cuda"), torch.ones((2, 6), device="cuda")
+    with pytest.raises(bz.BlazeHipError, match="act_params"):
+        bz.grouped_fc(a, w, cuts, 8, act=bz.ACT_DICE, act_params=(one, full, full))
+    with pytest.raises(bz.BlazeHipError, match="act_params"):
+        bz.fc_adapters(a, w[0], 8, _normal(2, (1, 3, 8)), _normal(3, (1, 6, 3)), torch.zeros(4, dtype=torch.int32, device="cuda"), act=bz.ACT_DICE,
+                       act_params=(one[0], full[0], full[0]))

@@ -888,15 +888,15 @@ def _code(who, name, t):
     return code
 
 
-def _act_fields(who, act_params, n, groups, here):
-    """(pointers of the activation's three parameters, how many of the first a group)"""
+def _act_fields(who, act, act_params, n, groups, here):
+    """(pointers of the activation's three parameters, how many of the first a group): n, or 1 of a PRelu's slopes"""
     if not act_params:
         return (0, 0, 0), 0
     p, first = [0, 0, 0], 0
     for i, t in enumerate(act_params[:3]):
         if t is not None:
             size = t.numel() // groups
-            if t.numel() != groups * size or (size != n and (i or size != 1)):
+            if t.numel() != groups * size or (size != n and (i or size != 1 or act != ACT_PRELU)):
                 raise BlazeHipError("%s: act_params[%d] has %d elements" % (who, i, t.numel()))
             p[i] = _vector(who, "act_params", t, _F32, t.numel(), here)
             first = size if i == 0 else first
@@ -920,7 +920,7 @@ def grouped_fc(a, w, offsets, k, rows=None, rows_per=1, bias=None, act=ACT_NONE,
         p_rows = _vector(who, "rows", rows, _I32, m, here)
     out = _empty((m, n), torch_dtype(out_dtype) if out_dtype else a.dtype, a, stream) if out is None else out
     p_y, ldy = _matrix(who, "out", out, None, (m, n), here)
-    p, act_size = _act_fields(who, act_params, n, groups, here)
+    p, act_size = _act_fields(who, act, act_params, n, groups, here)
     _call(lib().bz_grouped_fc, _GROUPED_FC_DESC.pack(p_a, p_rows, p_w, 0 if bias is None else _vector(who, "bias", bias, _F32, groups * cols, here), p_y,
                                                      _vector(who, "offsets", offsets, _I32, groups + 1, here), p[0], p[1], p[2], count, lda, ldw,
                                                      w_stride, ldy, m, n, k, groups, rows_per, _code(who, "a", a), _code(who, "out", out), act, act_size,
@@ -954,7 +954,7 @@ def fc_adapters(a, w, k, down, up, ids, rank=None, scale=None, bias=None, act=AC
         else:
             have = scratch.numel() * scratch.element_size()
             p_scratch = _vector(who, "scratch", scratch, scratch.dtype, scratch.numel(), here)
-    p, act_size = _act_fields(who, act_params, n, 1, here)
+    p, act_size = _act_fields(who, act, act_params, n, 1, here)
     _call(lib().bz_fc_adapters, _FC_ADAPTERS_DESC.pack(p_a, p_w, p_down, p_up, 0 if scale is None else _vector(who, "scale", scale, _F32, adapters, here),
                                                        _vector(who, "ids", ids, _I32, m, here),
                                                        0 if bias is None else _vector(who, "bias", bias, _F32, n, here), p_y, p[0], p[1], p[2], p_scratch,

@@ -1307,7 +1307,10 @@ inline int layer_act(const char* who, int act, int act_size, const float* p0, co
   BZ_REQUIRE(act == BZ_ACT_NONE || act == BZ_ACT_PRELU || act == BZ_ACT_DICE || act == BZ_ACT_LEAKY_RELU || act == BZ_ACT_SIGMOID,
              "%s: activation %d", who, act);
   if (act == BZ_ACT_PRELU) BZ_REQUIRE(p0 && (act_size == 1 || act_size == n), "%s: PRelu with %d slopes for %d columns", who, p0 ? act_size : 0, n);
-  if (act == BZ_ACT_DICE) BZ_REQUIRE(p0 && p1 && p2, "%s: Dice without its parameters", who);
+  if (act == BZ_ACT_DICE) {
+    BZ_REQUIRE(p0 && p1 && p2, "%s: Dice without its parameters", who);
+    BZ_REQUIRE(act_size == 0 || act_size == n, "%s: Dice with %d parameters for %d columns", who, act_size, n);
+  }
   return BZ_OK;
 }
 
