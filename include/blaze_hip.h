@@ -686,7 +686,7 @@ BZ_API int bz_merge_rows_grad(const bz_merge_grad_desc* desc, bz_stream_t stream
  *   y[r] = act( a[r] * w[g]^T + bias[g] )         or, with rows, a[rows[r] / rows_per] in place of a[r]
  * offsets and rows are bz_group_rows' (order, per).  w[g] is [n, ldw], K contiguous, as bz_fc_pack_weight lays a weight out;
  * groups follow at w_stride.  Rows of y at and behind offsets[groups] keep what they had.  A row index outside
- * [0, a_count) is a row of zeros.
+ * [0, a_count * rows_per) is a row of zeros.
  * act: any bz_act but the softmax, its parameters [groups, act_size] (PRelu, 1 or n) or [groups, n] (Dice, act_size n or 0); or BZ_ACT_SWIGLU:
  * w[g] is [2 * n, ldw] and bias [groups, 2 * n], and with v = a * w[g]^T + bias[g]
  *   y[r, c] = v[c] / (1 + e^-v[c]) * v[n + c]

@@ -864,3 +864,31 @@ def test_dice_of_one_parameter_a_group_is_refused(bz):
     with pytest.raises(bz.BlazeHipError, match="act_params"):
         bz.fc_adapters(a, w[0], 8, _normal(2, (1, 3, 8)), _normal(3, (1, 6, 3)), torch.zeros(4, dtype=torch.int32, device="cuda"), act=bz.ACT_DICE,
                        act_params=(one[0], full[0], full[0]))
+
+
+@pytest.mark.parametrize("m,n,k,groups,pad", ZERO_ROWS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+@pytest.mark.parametrize("per", [1, 2, 3])
+def test_grouped_fc_row_numbers_outside_are_rows_of_zeros(bz, m, n, k, groups, pad, dtype, act, per):
+    """-1, as a list is padded, and every other number below 0 or behind the last: as if `a` had a row of zeros there"""
+    import torch
+    print("case", m, n, k, groups, pad, dtype, act, per, flush=True)
+    source = 50
+    cols = 2 * n if act == "swiglu" else n
+    a, w, b = _normal(1, (source, k), 1.0, dtype), _pitched(_normal(2, (groups, cols, k), k**-0.5, dtype), pad, 0.0), _normal(3, (groups, cols), 0.1)
+    cuts = torch.tensor([m * g // groups for g in range(groups + 1)], dtype=torch.int32, device="cuda")
+    rng = np.random.default_rng(m + per)
+    rows = rng.integers(0, source * per, m).astype(np.int32)
+    outside = np.arange(m) % 3 == 1
+    rows[outside] = rng.choice([-1, 1 - per, -per, -per - 1, -1000, -2**31, source * per, source * per + per - 1, 2**31 - 1], outside.sum())
+    rows[outside & (rows == 0)] = -1  # (1 - per of one entry a row)
+    spare = torch.cat([a, torch.zeros((1, k), dtype=a.dtype, device="cuda")])
+    inside = torch.from_numpy(np.where(outside, source * per, rows).astype(np.int32)).cuda()
+    code = bz.ACT_SWIGLU if act == "swiglu" else bz.ACT_NONE
+    got = bz.grouped_fc(a, w, cuts, k, rows=torch.from_numpy(rows).cuda(), rows_per=per, bias=b, act=code)
+    want = bz.grouped_fc(spare, w, cuts, k, rows=inside, rows_per=per, bias=b, act=code)
+    assert torch.equal(got, want)
+    v = b.double().repeat_interleave(cuts[1:].long() - cuts[:-1].long(), 0)[torch.from_numpy(outside).cuda()]
+    zero = v[:, :n] * torch.sigmoid(v[:, :n]) * v[:, n:] if act == "swiglu" else v
+    _close(got[torch.from_numpy(outside).cuda()], zero, (HALF_STEP[dtype] + 32 * EPS) * zero.abs() + (2.0**-25 if dtype == "f16" else 0.0), "rows of zeros")

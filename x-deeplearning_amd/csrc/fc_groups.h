@@ -129,7 +129,10 @@ inline int64_t most_tiles(int64_t m, int groups, int bm) { return m / bm + std::
 // address of row r's input, null for a row of zeros
 __device__ __forceinline__ const char* input_row(const Layer& l, int r, int es) {
   int64_t at = r;
-  if (l.rows != nullptr) at = l.rows[r] / l.rows_per;
+  if (l.rows != nullptr) {
+    const int from = l.rows[r];
+    at = from < 0 ? -1 : from / l.rows_per;  // (a division alone makes row 0 of -1)
+  }
   return at >= 0 && at < l.a_count ? l.a + at * l.lda * es : nullptr;
 }
 
