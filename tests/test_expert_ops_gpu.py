@@ -251,3 +251,27 @@ def test_predictors_on_threads_of_their_own(pb):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_grouped_gemm_sigmoid_over_its_range(pb, dtype):
+    code = pb.K_FLOAT16 if dtype == np.float16 else pb.K_FLOAT
+    v = np.array([0.0, 1.0, -1.0, 20.0, -20.0, 88.0, 88.75, 89.0, -89.0, 120.0, 3e3, -3e3, 6e4, -6e4])
+    x, w = np.zeros((v.size, 8)), np.zeros((2, 8, 40))
+    x[:, 3], w[:, 3] = v, 1.0
+    nb = pb.NetBuilder("n", device_type=1)
+    nb.external_input("x", code)
+    nb.external_input("offsets", pb.K_INT32)
+    nb.external_output("y", code)
+    nb.constant("w", w.astype(np.float32), dtype=code)
+    nb.op("GroupedGemm", ["x", "w", "offsets"], ["y"], activation="sigmoid")
+    pm = pb.PredictorManager()
+    pm.load_model_from_string(nb.text(), True)
+    p = pm.create_predictor(1, 0)
+    p.feed("x", x.astype(dtype))
+    p.feed("offsets", np.array([0, 5, v.size], np.int32))
+    p.forward()
+    with np.errstate(over="ignore"):
+        want = np.broadcast_to((1.0 / (1.0 + np.exp(-v.astype(dtype).astype(np.float64))))[:, None], (v.size, 40))
+    bar = (_half(dtype) + 16 * EPS) * want + (2.0**-25 if dtype == np.float16 else 2.0**-126)
+    assert (np.abs(p.output_asnumpy("y").astype(np.float64) - want) <= bar).all()

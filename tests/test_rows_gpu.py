@@ -892,3 +892,62 @@ def test_grouped_fc_row_numbers_outside_are_rows_of_zeros(bz, m, n, k, groups, p
     v = b.double().repeat_interleave(cuts[1:].long() - cuts[:-1].long(), 0)[torch.from_numpy(outside).cuda()]
     zero = v[:, :n] * torch.sigmoid(v[:, :n]) * v[:, n:] if act == "swiglu" else v
     _close(got[torch.from_numpy(outside).cuda()], zero, (HALF_STEP[dtype] + 32 * EPS) * zero.abs() + (2.0**-25 if dtype == "f16" else 0.0), "rows of zeros")
+
+
+# ---------------------------------------------------------------------------------------------- activations over all of their range
+def _values(dtype):
+    """pre-activations over the range that any type has: small, large, either sign"""
+    v = [0.0, 1.0, -1.0, 0.25, 8.0, -8.0, 20.0, -20.0, 60.0, -60.0, 88.0, -88.0, 88.75, -88.75, 89.0, 100.0, -100.0, 104.0, 300.0, -300.0, 5e3, -5e3, 6e4, -6e4]
+    return v + ([1e30, -1e30, 3e38, -3e38] if dtype != "f16" else []) + [float("inf"), float("-inf"), float("nan")]
+
+
+# (rows, elements between rows of w beyond K) at N 1100, K 64: the kernel for few rows, the one for rows that begin anywhere, the one for many rows
+BY_KERNEL = [(20, 0), (3000, 1), (3000, 0)]
+
+
+def _spread(bz, m, pad, dtype, groups, n=1100, k=64):
+    """an `a` and a `w` whose products are exactly the values of _values, one a row: (a, w, cuts, v [m, n] in 64 bits)"""
+    import torch
+    values = torch.tensor(_values(dtype), dtype=torch.float64, device="cuda").to(_t(dtype))
+    a = torch.zeros((m, k), dtype=_t(dtype), device="cuda")
+    at = torch.arange(m, device="cuda") % values.numel()
+    a[:, 5] = values[at]
+    w = torch.zeros((groups, n, k), dtype=_t(dtype), device="cuda")
+    w[:, :, 5] = 1.0
+    cuts = torch.tensor([m * g // groups for g in range(groups + 1)], dtype=torch.int32, device="cuda")
+    return a, _pitched(w, pad, 0.0), cuts, values[at].double()[:, None].expand(m, n)
+
+
+@pytest.mark.parametrize("m,pad", BY_KERNEL)
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_sigmoid_layers_over_their_range(bz, m, pad, dtype, out):
+    """every pre-activation has its sigmoid, infinities among them"""
+    import torch
+    code = {"f32": bz.F32, "f16": bz.F16, "bf16": bz.BF16}[out]
+    a, w, cuts, v = _spread(bz, m, pad, dtype, 3)
+    some = torch.isfinite(v)
+    want = torch.sigmoid(v)
+    # exp of an exact argument, a sum and a division, rounded once; what is below 2^-126 may be flushed
+    bar = (HALF_STEP[out] + 16 * EPS) * want.nan_to_num(0.0) + (2.0**-25 if out == "f16" else 2.0**-126)
+    y = bz.grouped_fc(a, w, cuts, 64, act=bz.ACT_SIGMOID, out_dtype=code)
+    _close(y, want, bar, "grouped")
+    z = bz.fc_adapters(a, w[0], 64, torch.zeros((2, 8, 64), dtype=a.dtype, device="cuda"), torch.zeros((2, 1100, 8), dtype=a.dtype, device="cuda"),
+                       (torch.arange(m, device="cuda") % 3 - 1).to(torch.int32), act=bz.ACT_SIGMOID, out_dtype=code)
+    _close(z[some], want[some], bar[some], "adapters")  # (an infinity times down's zeros is none of them)
+
+
+@pytest.mark.parametrize("m,pad", BY_KERNEL)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_sigmoid_layers_of_infinite_sums(bz, m, pad, dtype):
+    """a bias of either infinity is an infinite pre-activation, whose sigmoid is 1 or 0"""
+    import torch
+    a, w, cuts, _ = _spread(bz, m, pad, dtype, 2)
+    a.fill_(0.5)
+    bias = torch.zeros((2, 1100), device="cuda")
+    bias[0, ::2], bias[1, ::3] = float("inf"), float("-inf")
+    y = bz.grouped_fc(a, w, cuts, 64, bias=bias, act=bz.ACT_SIGMOID)
+    half = torch.sigmoid(torch.tensor(0.5, dtype=torch.float64)).item()
+    cut = int(cuts[1])
+    want = torch.full((m, 1100), half, dtype=torch.float64, device="cuda")
+    want[:cut, ::2], want[cut:, ::3] = 1.0, 0.0
+    _close(y, want, (HALF_STEP[dtype] + 16 * EPS) * want, "y")

@@ -258,6 +258,13 @@ __device__ __forceinline__ void add_adapters(const Layer& l, int id, int row0, i
   }
 }
 
+// The layers' activation.  Sigmoid is 1 / (1 + e^-v), which has a value for any v; the shared layers' e^v / (1 + e^v) is NaN from v = 88.73 on.
+template <int ACT>
+__device__ __forceinline__ float activated(float v, const bz::fc::Epilogue& ep, float p0, float p1, float p2) {
+  if constexpr (ACT == BZ_ACT_SIGMOID) return 1.f / (1.f + expf(-v));
+  return bz::fc::apply_act_t<ACT>(v, ep, p0, p1, p2);
+}
+
 // The parameters of column c of group g
 template <int ACT>
 struct Column {
@@ -274,7 +281,7 @@ struct Column {
     }
   }
   __device__ __forceinline__ float of(const Layer& l, float v) const {
-    return bz::fc::apply_act_t<ACT>(fmaf(l.ep.alpha, v, bias), l.ep, p0, p1, p2);
+    return activated<ACT>(fmaf(l.ep.alpha, v, bias), l.ep, p0, p1, p2);
   }
 };
 
@@ -402,7 +409,7 @@ __global__ __launch_bounds__(256) void bz_groups_tile_kernel(Layer l, int tiles_
           if constexpr (GATED)
             v = silu(acc[i][0][r] + gate_bias) * (acc[i][TN - 1][r] + up_bias);
           else if constexpr (ADAPTERS)
-            v = bz::fc::apply_act_t<ACT>(acc[i][j][r] + p.bias, l.ep, p.p0, p.p1, p.p2);
+            v = activated<ACT>(acc[i][j][r] + p.bias, l.ep, p.p0, p.p1, p.p2);
           else
             v = p.of(l, acc[i][j][r]);
           if (row < m1 && col < l.n) put_out<DT>(l, (int64_t)row * l.ldy + col, v);
@@ -649,7 +656,7 @@ __global__ __launch_bounds__(NW * 64) void bz_groups_split_kernel(Layer l, int t
       if constexpr (GATED)
         v = silu(sum(r, c) + bias) * (sum(r, c + 16) + p0);
       else
-        v = bz::fc::apply_act_t<ACT>(ADAPTERS ? sum(r, c) + b : fmaf(l.ep.alpha, sum(r, c), b), l.ep, p0, p1, q2);
+        v = activated<ACT>(ADAPTERS ? sum(r, c) + b : fmaf(l.ep.alpha, sum(r, c), b), l.ep, p0, p1, q2);
       put_out<DT>(l, (int64_t)(m0 + r) * l.ldy + col, v);
     }
   };
@@ -1134,7 +1141,7 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
         if constexpr (GATED)
           y[x] = silu(sum + bias[x]) * ((there ? v[x + 32] : 0.f) + p0[x]);
         else
-          y[x] = bz::fc::apply_act_t<ACT>(ADAPTERS ? sum + bias[x] : fmaf(l.ep.alpha, sum, bias[x]), l.ep, p0[x], p1[x], p2[x]);
+          y[x] = activated<ACT>(ADAPTERS ? sum + bias[x] : fmaf(l.ep.alpha, sum, bias[x]), l.ep, p0[x], p1[x], p2[x]);
       }
       OutT* to = out + (int64_t)(row + r) * l.ldy + col;
       if (fast) {
