@@ -951,3 +951,25 @@ def test_sigmoid_layers_of_infinite_sums(bz, m, pad, dtype):
     want = torch.full((m, 1100), half, dtype=torch.float64, device="cuda")
     want[:cut, ::2], want[cut:, ::3] = 1.0, 0.0
     _close(y, want, (HALF_STEP[dtype] + 16 * EPS) * want, "y")
+
+
+@pytest.mark.parametrize("m,pad", BY_KERNEL)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("slope", [0.0, 0.25])
+def test_relu_layers_over_their_range(bz, m, pad, dtype, slope):
+    """-infinity is 0 with a slope of 0, and a NaN stays one"""
+    import torch
+    a, w, cuts, v = _spread(bz, m, pad, dtype, 3)
+    y = bz.grouped_fc(a, w, cuts, 64, act=bz.ACT_LEAKY_RELU, act_alpha=slope)
+    want = torch.where(v >= 0, v, torch.nan_to_num(slope * v, nan=0.0, neginf=-float("inf")))
+    want = torch.where(torch.isnan(v), v, want)
+    _close(y, want, (HALF_STEP[dtype] + EPS) * want.nan_to_num(0.0, 0.0, 0.0).abs(), "y")
+    bias = torch.zeros((3, 1100), device="cuda")
+    bias[:, ::2] = -float("inf")
+    a.fill_(0.5)
+    z = bz.grouped_fc(a, w, cuts, 64, bias=bias, act=bz.ACT_LEAKY_RELU, act_alpha=slope)
+    assert bool((z[:, ::2] == (0.0 if slope == 0 else -float("inf"))).all()) and bool((z[:, 1::2] == 0.5).all())
+    ids = (torch.arange(m, device="cuda") % 3 - 1).to(torch.int32)
+    z = bz.fc_adapters(a, w[0], 64, torch.zeros((2, 8, 64), dtype=a.dtype, device="cuda"), torch.zeros((2, 1100, 8), dtype=a.dtype, device="cuda"), ids,
+                       bias=bias[0].contiguous(), act=bz.ACT_LEAKY_RELU, act_alpha=slope)
+    assert bool((z[:, ::2] == (0.0 if slope == 0 else -float("inf"))).all()) and bool((z[:, 1::2] == 0.5).all())

@@ -259,9 +259,11 @@ __device__ __forceinline__ void add_adapters(const Layer& l, int id, int row0, i
 }
 
 // The layers' activation.  Sigmoid is 1 / (1 + e^-v), which has a value for any v; the shared layers' e^v / (1 + e^v) is NaN from v = 88.73 on.
+// A leaky ReLU of slope 0 is ReLU: 0 below 0, where the product with -infinity is NaN.
 template <int ACT>
 __device__ __forceinline__ float activated(float v, const bz::fc::Epilogue& ep, float p0, float p1, float p2) {
   if constexpr (ACT == BZ_ACT_SIGMOID) return 1.f / (1.f + expf(-v));
+  if constexpr (ACT == BZ_ACT_LEAKY_RELU) return v >= 0.f ? v : v < 0.f && ep.act_alpha == 0.f ? 0.f : ep.act_alpha * v;
   return bz::fc::apply_act_t<ACT>(v, ep, p0, p1, p2);
 }
 
