@@ -973,3 +973,41 @@ def test_relu_layers_over_their_range(bz, m, pad, dtype, slope):
     z = bz.fc_adapters(a, w[0], 64, torch.zeros((2, 8, 64), dtype=a.dtype, device="cuda"), torch.zeros((2, 1100, 8), dtype=a.dtype, device="cuda"), ids,
                        bias=bias[0].contiguous(), act=bz.ACT_LEAKY_RELU, act_alpha=slope)
     assert bool((z[:, ::2] == (0.0 if slope == 0 else -float("inf"))).all()) and bool((z[:, 1::2] == 0.5).all())
+
+
+@pytest.mark.parametrize("m,pad", BY_KERNEL)
+@pytest.mark.parametrize("nosqrt", [True, False])
+def test_fp32_dice_far_from_its_mean(bz, m, pad, nosqrt):
+    """Far below the mean Dice is e^(v - mean) v and little else: pre-activations that are exact, a deviation of 1, so that what is off
+    is the activation's own arithmetic.  Rounded: v - mean and its quotient not at all (small whole numbers and quarters over 1), exp by 2 steps,
+    1 + t, 1 / that, two products and a sum by one each; 16 steps in all."""
+    import torch
+    n, k, groups = 1100, 64, 2
+    a = torch.zeros((m, k), device="cuda")
+    a[:, 9] = -(torch.arange(m, device="cuda") % 280) / 4.0
+    w = torch.zeros((groups, n, k), device="cuda")
+    w[:, :, 9] = 1.0
+    cuts = torch.tensor([0, m // 3, m], dtype=torch.int32, device="cuda")
+    gamma, mean, var = torch.zeros((groups, n), device="cuda"), torch.full((groups, n), 2.0, device="cuda"), torch.ones((groups, n), device="cuda")
+    y = bz.grouped_fc(a, _pitched(w, pad, 0.0), cuts, k, act=bz.ACT_DICE, act_params=(gamma, mean, var), dice_nosqrt=nosqrt)
+    v = a[:, 9].double()[:, None].expand(m, n)
+    want = torch.sigmoid(v - 2.0) * v  # (sqrt(1 + 1e-8) is 1 in fp32)
+    _close(y, want, 16 * EPS * want.abs(), "grouped")
+    z = bz.fc_adapters(a, _pitched(w, pad, 0.0)[0], k, torch.zeros((1, 4, k), device="cuda"), torch.zeros((1, n, 4), device="cuda"),
+                       torch.zeros(m, dtype=torch.int32, device="cuda"), act=bz.ACT_DICE, act_params=(gamma[0], mean[0], var[0]), dice_nosqrt=nosqrt)
+    _close(z, want, 16 * EPS * want.abs(), "adapters")
+
+
+@pytest.mark.parametrize("m,pad", BY_KERNEL)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_dice_of_infinite_sums(bz, m, pad, dtype):
+    """v above, gamma * v below: infinities where those are"""
+    import torch
+    n, k, groups = 1100, 64, 2
+    a, w = torch.full((m, k), 0.5, dtype=_t(dtype), device="cuda"), torch.zeros((groups, n, k), dtype=_t(dtype), device="cuda")
+    bias = torch.zeros((groups, n), device="cuda")
+    bias[:, ::3], bias[:, 1::3] = float("inf"), -float("inf")
+    params = torch.full((groups, n), 0.5, device="cuda"), torch.zeros((groups, n), device="cuda"), torch.ones((groups, n), device="cuda")
+    cuts = torch.tensor([0, m // 3, m], dtype=torch.int32, device="cuda")
+    y = bz.grouped_fc(a, _pitched(w, pad, 0.0), cuts, k, bias=bias, act=bz.ACT_DICE, act_params=params)
+    assert bool((y[:, ::3] == float("inf")).all()) and bool((y[:, 1::3] == -float("inf")).all()) and bool((y[:, 2::3] == 0).all())

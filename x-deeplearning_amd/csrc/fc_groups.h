@@ -259,16 +259,27 @@ __device__ __forceinline__ void add_adapters(const Layer& l, int id, int row0, i
 }
 
 // The layers' activation.  Sigmoid is 1 / (1 + e^-v), which has a value for any v; the shared layers' e^v / (1 + e^v) is NaN from v = 88.73 on.
-// A leaky ReLU of slope 0 is ReLU: 0 below 0, where the product with -infinity is NaN.
-template <int ACT>
+// A leaky ReLU of slope 0 is ReLU: 0 below 0, where the product with -infinity is NaN.  fp32 layers have an exact Dice, whose error does not
+// grow as fast with the distance from the mean (v_exp_f32's argument, rounded after a product with log2(e), is 2^-24 of itself off: 60
+// deviations from the mean 60 steps of the result).  p2 is what dice_column makes of a column's variance.
+template <int DT, int ACT>
 __device__ __forceinline__ float activated(float v, const bz::fc::Epilogue& ep, float p0, float p1, float p2) {
+  if constexpr (DT == BZ_F32 && ACT == BZ_ACT_DICE) {
+    const float p = 1.f / (1.f + expf((p1 - v) / p2));
+    return fmaf(1.f - p, p0, p) * v;
+  }
   if constexpr (ACT == BZ_ACT_SIGMOID) return 1.f / (1.f + expf(-v));
   if constexpr (ACT == BZ_ACT_LEAKY_RELU) return v >= 0.f ? v : v < 0.f && ep.act_alpha == 0.f ? 0.f : ep.act_alpha * v;
   return bz::fc::apply_act_t<ACT>(v, ep, p0, p1, p2);
 }
 
+template <int DT>
+__device__ __forceinline__ float dice_column(const bz::fc::Epilogue& ep, float var) {
+  return DT == BZ_F32 ? bz::fc::dice_den(ep, var) : bz::fc::dice_inv_den(ep, var);
+}
+
 // The parameters of column c of group g
-template <int ACT>
+template <int DT, int ACT>
 struct Column {
   float bias = 0.f, p0 = 0.f, p1 = 0.f, p2 = 0.f;
   __device__ __forceinline__ Column(const Layer& l, int g, int c, int bias_cols) {
@@ -279,11 +290,11 @@ struct Column {
     if constexpr (ACT == BZ_ACT_DICE) {
       p0 = ep.p0[p + c];
       p1 = ep.p1[p + c];
-      p2 = bz::fc::dice_inv_den(ep, ep.p2[p + c]);
+      p2 = dice_column<DT>(ep, ep.p2[p + c]);
     }
   }
   __device__ __forceinline__ float of(const Layer& l, float v) const {
-    return activated<ACT>(fmaf(l.ep.alpha, v, bias), l.ep, p0, p1, p2);
+    return activated<DT, ACT>(fmaf(l.ep.alpha, v, bias), l.ep, p0, p1, p2);
   }
 };
 
@@ -400,7 +411,7 @@ __global__ __launch_bounds__(256) void bz_groups_tile_kernel(Layer l, int tiles_
 #pragma unroll
     for (int j = 0; j < COLS; ++j) {
       const int col = col0 + j * 32 + frow, cc = min(col, l.n - 1);
-      const Column<ACT> p(l, group, cc, GATED ? 2 * l.n : l.n);
+      const Column<DT, ACT> p(l, group, cc, GATED ? 2 * l.n : l.n);
       const float gate_bias = p.bias, up_bias = GATED && l.ep.bias != nullptr ? l.ep.bias[(int64_t)group * 2 * l.n + l.n + cc] : 0.f;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -411,7 +422,7 @@ __global__ __launch_bounds__(256) void bz_groups_tile_kernel(Layer l, int tiles_
           if constexpr (GATED)
             v = silu(acc[i][0][r] + gate_bias) * (acc[i][TN - 1][r] + up_bias);
           else if constexpr (ADAPTERS)
-            v = activated<ACT>(acc[i][j][r] + p.bias, l.ep, p.p0, p.p1, p.p2);
+            v = activated<DT, ACT>(acc[i][j][r] + p.bias, l.ep, p.p0, p.p1, p.p2);
           else
             v = p.of(l, acc[i][j][r]);
           if (row < m1 && col < l.n) put_out<DT>(l, (int64_t)row * l.ldy + col, v);
@@ -652,13 +663,13 @@ __global__ __launch_bounds__(NW * 64) void bz_groups_split_kernel(Layer l, int t
   auto finish = [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     if (col >= l.n) return;
-    const float q2 = ACT == BZ_ACT_DICE ? bz::fc::dice_inv_den(l.ep, p2) : 0.f, b = l.ep.beta * bias;
+    const float q2 = ACT == BZ_ACT_DICE ? dice_column<DT>(l.ep, p2) : 0.f, b = l.ep.beta * bias;
     for (int r = tid / OUT; r < 32 && m0 + r < m1; r += NW * 64 / OUT) {
       float v;
       if constexpr (GATED)
         v = silu(sum(r, c) + bias) * (sum(r, c + 16) + p0);
       else
-        v = activated<ACT>(ADAPTERS ? sum(r, c) + b : fmaf(l.ep.alpha, sum(r, c), b), l.ep, p0, p1, q2);
+        v = activated<DT, ACT>(ADAPTERS ? sum(r, c) + b : fmaf(l.ep.alpha, sum(r, c), b), l.ep, p0, p1, q2);
       put_out<DT>(l, (int64_t)(m0 + r) * l.ldy + col, v);
     }
   };
@@ -842,7 +853,7 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
     params[tid] = ep.bias != nullptr ? ep.beta * ep.bias[(int64_t)group * (GATED ? 2 * l.n : l.n) + col] : 0.f;
     params[BN + tid] = !GATED && (ep.act == BZ_ACT_PRELU || dice) ? ep.p0[at] : 0.f;
     params[2 * BN + tid] = dice ? ep.p1[at] : 0.f;
-    params[3 * BN + tid] = dice ? bz::fc::dice_inv_den(ep, ep.p2[at]) : 0.f;
+    params[3 * BN + tid] = dice ? dice_column<DT>(ep, ep.p2[at]) : 0.f;
   }
   if (tid < BM) {
     const int row = min(m0 + tid, m1 - 1);
@@ -1143,7 +1154,7 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
         if constexpr (GATED)
           y[x] = silu(sum + bias[x]) * ((there ? v[x + 32] : 0.f) + p0[x]);
         else
-          y[x] = activated<ACT>(ADAPTERS ? sum + bias[x] : fmaf(l.ep.alpha, sum, bias[x]), l.ep, p0[x], p1[x], p2[x]);
+          y[x] = activated<DT, ACT>(ADAPTERS ? sum + bias[x] : fmaf(l.ep.alpha, sum, bias[x]), l.ep, p0[x], p1[x], p2[x]);
       }
       OutT* to = out + (int64_t)(row + r) * l.ldy + col;
       if (fast) {
