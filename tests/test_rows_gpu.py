@@ -1011,3 +1011,68 @@ def test_dice_of_infinite_sums(bz, m, pad, dtype):
     cuts = torch.tensor([0, m // 3, m], dtype=torch.int32, device="cuda")
     y = bz.grouped_fc(a, _pitched(w, pad, 0.0), cuts, k, bias=bias, act=bz.ACT_DICE, act_params=params)
     assert bool((y[:, ::3] == float("inf")).all()) and bool((y[:, 1::3] == -float("inf")).all()) and bool((y[:, 2::3] == 0).all())
+
+
+@pytest.mark.parametrize("scale_a,scale_w", [(2.0**-124, 1.0), (2.0**-124, 2.0**20), (2.0**-124, 2.0**60), (2.0**-118, 2.0**60), (2.0**-124, 2.0**110), (2.0**60, 2.0**-124),
+                                             (2.0**20, 2.0**-124), (2.0**-60, 2.0**-50), (1.0, 2.0**-120)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k,groups", [(2500, 700, 200, 3), (30, 700, 200, 3)])
+def test_grouped_fc_fp32_of_very_small_operands(bz, scale_a, scale_w, gated, m, n, k, groups):
+    """Some rows so small that a split in pieces drops bits of them, beside ordinary ones, in long batches and short ones: fp32 sums like any
+    other, (K + 8) * 2^-24 of their terms, and 2^-126 for what may be flushed of each product."""
+    import torch
+    cols = 2 * n if gated else n
+    small = torch.arange(m, device="cuda") % 5 == 2
+    a, w = _normal(0, (m, k)), _normal(1, (groups, cols, k), 1.0 / np.sqrt(k))
+    small_cols = torch.arange(cols, device="cuda") % 7 == 3
+    # (1 and more, so that no operand is below 2^-126 itself)
+    a[small] = torch.sign(a[small]) * (1.0 + a[small].abs()) * scale_a
+    w[:, small_cols] = torch.sign(w[:, small_cols]) * (1.0 + w[:, small_cols].abs()) * scale_w
+    cuts = torch.tensor([m * g // groups for g in range(groups + 1)], dtype=torch.int32, device="cuda")
+    if gated:  # up: the gate is one half of a row's first input, so that silu(gate) * up is linear in up
+        a[:, 0] = 2.0
+        w[:, :n] = 0.0
+        w[:, :n, 0] = 0.5  # gate 1 in every row
+        w[:, n:, 0] = 0.0
+        y = bz.grouped_fc(a, w, cuts, k, act=bz.ACT_SWIGLU).double()
+        factor = float(torch.sigmoid(torch.tensor(1.0, dtype=torch.float64)))
+        w = w[:, n:]
+    else:
+        y, factor = bz.grouped_fc(a, w, cuts, k).double(), 1.0
+    for g in range(groups):
+        lo, hi = int(cuts[g]), int(cuts[g + 1])
+        x, v = a[lo:hi].double(), w[g].double()
+        want, size = x @ v.t(), x.abs() @ v.abs().t()
+        _close(y[lo:hi], factor * want, factor * ((k + 8) * EPS * size + k * 2.0**-126) + 32 * EPS * want.abs(), "group %d" % g)
+
+
+def test_fc_adapters_fp32_of_very_small_operands(bz):
+    import torch
+    m, n, k, rank = 2500, 1000, 200, 8
+    a, w = _normal(0, (m, k)), _normal(1, (n, k), 2.0**20 / np.sqrt(k))
+    a[::5] = torch.sign(a[::5]) * (1.0 + a[::5].abs()) * 2.0**-124
+    down, up = _normal(2, (2, rank, k), 2.0**20 / np.sqrt(k)), _normal(3, (2, n, rank))
+    ids = (torch.arange(m, device="cuda") % 3 - 1).to(torch.int32)
+    y = bz.fc_adapters(a, w, k, down, up, ids)
+    x = a.double()
+    want, size = x @ w.double().t(), x.abs() @ w.double().abs().t()
+    for g in range(2):
+        r = ids == g
+        want[r] += (x[r] @ down[g].double().t()) @ up[g].double().t()
+        size[r] += (x[r].abs() @ down[g].double().abs().t()) @ up[g].double().abs().t()
+    _close(y, want, (k + 3 * rank + 24) * EPS * size + (k + rank) * 2.0**-126 * 2.0**4, "y")
+
+
+def test_grouped_fc_fp32_results_do_not_depend_on_a_row_of_zeros_or_large_ones(bz):
+    """rows beside rows of zeros, of very large numbers and of infinities are bit for bit what they are without them"""
+    import torch
+    m, n, k = 2500, 700, 200
+    a, w = _normal(0, (m, k)), _normal(1, (2, n, k), 1.0 / np.sqrt(k))
+    cuts = torch.tensor([0, 1000, m], dtype=torch.int32, device="cuda")
+    a[::3] *= 2.0**-60
+    want = bz.grouped_fc(a, w, cuts, k)
+    other = torch.arange(m, device="cuda") % 64 == 17
+    for value in (0.0, 1e30, float("inf")):
+        b = a.clone()
+        b[other] = value
+        assert torch.equal(bz.grouped_fc(b, w, cuts, k)[~other], want[~other])

@@ -918,22 +918,6 @@ __device__ __forceinline__ void load_to_lds_from(const char* base, uint32_t off,
                : "memory", "m0", "scc");
 }
 
-// m = the largest of m, |x| and |y|.  (NaNs are passed over, and make their sums NaNs anyway.  In assembly, so that it stands where the
-// products have ended: alternated with them, 2048 x 896 -> 512 took 0.8 us more.)
-__device__ __forceinline__ void largest(float& m, float x, float y) { asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y)); }
-// Whether a sum of K split products may be off, max_a and max_w being the largest |operands| of its two rows: it is not finite, or so
-// small that what a split may drop of operands below 2^-110, at most 2^-126 of each, times the other row's largest counts in it.
-// (What the matrix instructions may flush of the products, 2^-126 of each of the six, is less than that for 1.)
-constexpr float kSplitDrops = 0x1p-98f;
-__device__ __forceinline__ bool doubtful(float v, int K, float max_a, float max_w) {
-  const float least = (float)K * kSplitDrops * fmaxf(1.f, fmaxf(max_a, max_w));
-  const bool off = !(fabsf(v) >= least && fabsf(v) < __builtin_huge_valf());
-  return off && !(v == 0.f && (max_a == 0.f || max_w == 0.f));
-}
-// Where no operand of a tile is beyond this, and no sum of it doubtful for this, nothing is: one look at the tile.  (Each sum by its own
-// rows' largest operands, without it, made 2048 x 896 -> 512 16.9 us, the tile's at once 16.0; without any of this it was 15.8.)
-constexpr float kOrdinary = 0x1p40f;
-
 // EXACT: Dice as apply_act computes it, not as the tile kernels do
 template <typename OutT, int NW, int TM, int TN, int SUMS, bool EXACT>
 __global__ __launch_bounds__(NW * 64, 2) void bz_fc_f32_kernel(const char* __restrict__ A, const char* __restrict__ W, int M, int N, int K,

@@ -978,11 +978,12 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
   // 32x32x16 where the fp32 instructions take 512.  An operand is converted once for all four waves, on its way to LDS: it comes through
   // registers, two stages ahead, and a stage's pieces lie in one of two places as three matrices of 64 bytes a row, chunk c of row r at
   // position c ^ ((r >> 2) & 3).  Bound by the conversions and the instructions that feed the matrix cores: 8192 rows, 2048 -> 2048 475 us, 145
-  // TFLOP/s (730 with fp32 instructions, in the tile kernel); 2048 x 2 rows of 896 -> 512 through 8 experts 40.6 (44.7 with each wave converting
+  // TFLOP/s (730 with fp32 instructions, in the tile kernel); 2048 x 2 rows of 896 -> 512 through 8 experts 40.6 without what finds doubtful sums (44.7 with each wave converting
   // the fragments that it read).
-  // An operand below 2^-110 is off by up to 2^-126; one that is no number, infinite or within 2^-9 of it makes sums that are not finite: the
+  // A sum that is not finite, or small enough that what a split drops of its operands may count in it, is doubtful (bz::fc::doubtful): the
   // tile is multiplied again with fp32 instructions then, and such sums are taken from there (the others stay, so that no row's result
-  // depends on what is in another).
+  // depends on what is in another).  For that the largest operand of each row is kept on the way (2048 x 2 rows of 896 -> 512: 40.6 -> 41.5 us).
+  uint32_t again[TM][TN];  // the doubtful ones of a block's sums
   auto multiply_split = [&]() {
     using bz::fc::Bf16x3;
     constexpr int ITEMS = ROWS / 64, PLANE = ROWS * 64;  // eight floats an item
@@ -1011,8 +1012,16 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
           }
       }
     };
+    float most[ITEMS];  // the largest |operand| that the thread has seen of the item's row
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) most[q] = 0.f;
     auto put = [&](const Raw& from, int place, int q) {
       const Bf16x3 v = bz::fc::split_floats(from.x[q][0], from.x[q][1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        bz::fc::largest(most[q], __uint_as_float(from.x[q][c].x), __uint_as_float(from.x[q][c].y));
+        bz::fc::largest(most[q], __uint_as_float(from.x[q][c].z), __uint_as_float(from.x[q][c].w));
+      }
       const int row = q * 64 + irow;
       char* to = smem + place * (3 * PLANE) + row * 64 + ((ichunk ^ ((row >> 2) & 3)) << 4);
       *(uint4*)to = v.hi;
@@ -1048,7 +1057,7 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
     };
     // a step's products, and between them the conversion of items from..to
     auto step = [&](const Pieces& p, const Raw& r, int place, auto from_c, auto to_c) {
-      constexpr int FROM = decltype(from_c)::value, TO = decltype(to_c)::value, MFMAS = 6 * BLOCKS, EACH = ((TO - FROM) * 50 + MFMAS - 1) / MFMAS;
+      constexpr int FROM = decltype(from_c)::value, TO = decltype(to_c)::value, MFMAS = 6 * BLOCKS, EACH = ((TO - FROM) * 54 + MFMAS - 1) / MFMAS;
       __builtin_amdgcn_sched_barrier(0);
       products(p);
 #pragma unroll
@@ -1091,13 +1100,36 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
     }
     if (i < stages) stage(i, std::integral_constant<int, 0>());
     __syncthreads();
-    bool off = false;
+    // the rows' largest operands, where the stages were: four threads have seen parts of a row
+    float* row_most = (float*)smem;
+    bool look = false;
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      most[q] = fmaxf(most[q], __shfl_xor(most[q], 1));
+      most[q] = fmaxf(most[q], __shfl_xor(most[q], 2));
+      if (ichunk == 0) row_most[q * 64 + irow] = most[q];
+      look |= most[q] > bz::fc::kOrdinary;
+    }
+    const float least = (float)l.k * (bz::fc::kSplitDrops * bz::fc::kOrdinary);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) off |= !(fabsf(acc[i][j][r]) < __builtin_huge_valf());
+        for (int r = 0; r < 16; ++r) look |= !(fabsf(acc[i][j][r]) >= least && fabsf(acc[i][j][r]) < __builtin_huge_valf());
+    if (__syncthreads_or(look) == 0) return false;
+    bool off = false;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        again[i][j] = 0;
+        const float max_w = row_most[BM + wn * 32 * TN + j * 32 + frow];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          again[i][j] |= bz::fc::doubtful(acc[i][j][r], l.k, row_most[block_row(i) + 8 * (r >> 2) + 4 * half + (r & 3)], max_w) ? 1u << r : 0u;
+        off |= again[i][j] != 0;
+      }
     return __syncthreads_or(off) != 0;
   };
   if constexpr (DT == BZ_F32) {
@@ -1113,7 +1145,7 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = fabsf(split[i][j][r]) < __builtin_huge_valf() ? split[i][j][r] : acc[i][j][r];
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = again[i][j] >> r & 1 ? acc[i][j][r] : split[i][j][r];
     }
   } else {
     multiply();
