@@ -721,7 +721,7 @@ BZ_API int bz_grouped_fc(const bz_grouped_fc_desc* desc, bz_stream_t stream);
  * A layer that all rows share, and beside it each row's own low-rank product:
  *   y[r] = act( alpha * a[r] * w^T + scale[g] * (a[r] * down[g]^T) * up[g]^T + beta * bias ),  g = ids[r]
  * A row whose id is outside [0, adapters) has no adapter.  The low-rank product between the two factors is kept to 16 bits of
- * mantissa or more (two bf16s, or fp32 for fp32 layers); what one row's adapter holds reaches no other row.  Adapters of a lower rank
+ * mantissa or more (two bf16s, or fp32 for fp32 layers), infinities as they are in fp32; what one row's adapter holds reaches no other row.  Adapters of a lower rank
  * than `rank` are filled up with zeros.  Rows of one adapter cost least next to each other.
  * scratch: m * bz_fc_adapters_scratch_bytes(1, rank) bytes, needed where adapters > 0.
  */

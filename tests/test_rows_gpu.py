@@ -1076,3 +1076,54 @@ def test_grouped_fc_fp32_results_do_not_depend_on_a_row_of_zeros_or_large_ones(b
         b = a.clone()
         b[other] = value
         assert torch.equal(bz.grouped_fc(b, w, cuts, k)[~other], want[~other])
+
+
+# ---------------------------------------------------------------------------------------------- adapters of infinities
+def _bounds_case(bz, m, pad, dtype, rank, adapters, n=700, k=64):
+    """positive operands of an adapter layer, so that no infinity meets another one's opposite; w at another pitch by `pad`"""
+    import torch
+    a, w = _normal(0, (m, k), 1.0, dtype).abs() + 0.25, _normal(1, (n, k), k**-0.5, dtype).abs()
+    down, up = _normal(2, (adapters, rank, k), k**-0.5, dtype).abs() + 2.0**-6, _normal(3, (adapters, n, rank), rank**-0.5, dtype).abs() + 2.0**-6
+    return a, _pitched(w, pad, 0.0), down, up
+
+
+def _adapters_want(a, w, down, up, ids):
+    """in 64 bits, a product and a sum at a time, so that what is no number comes as it does by IEEE"""
+    import torch
+    y = (a.double()[:, None, :] * w.double()[None]).sum(2)
+    for g in range(down.shape[0]):
+        r = torch.nonzero(ids == g)[:, 0]
+        if r.numel():
+            low = (a[r].double()[:, None, :] * down[g].double()[None]).sum(2)
+            y[r] += (low[:, None, :] * up[g].double()[None]).sum(2)
+    return y
+
+
+@pytest.mark.parametrize("m,pad", [(20, 0), (900, 1), (900, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [16, 32, 48])
+def test_fc_adapters_of_infinite_weights(bz, m, pad, dtype, rank):
+    """an infinity of either sign in `up` is one in the rows of its adapter, and one in a row's factor is one there: no NaNs"""
+    import torch
+    print("case", m, pad, dtype, rank, flush=True)
+    inf = float("inf")
+    a, w, down, up = _bounds_case(bz, m, pad, dtype, rank, 3)
+    ids = (torch.arange(m, device="cuda") // 7 % 4 - 1).to(torch.int32)
+    up[0, 5, 3], up[1, 6, rank - 1], up[2, 650, 0], up[2, 651, 9] = inf, -inf, inf, float("nan")
+    want = _adapters_want(a, w, down, up, ids)
+    got = bz.fc_adapters(a, w, 64, down, up, ids).double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and int(torch.isnan(want).sum()) == int((ids == 2).sum())
+    far = torch.isinf(want)
+    assert int(far.sum()) == int((ids >= 0).sum()) and bool((got[far] == want[far]).all())
+    near = torch.isfinite(want)
+    _close(got[near], want[near], (HALF_STEP[dtype] + 2.0**-15) * want[near].abs(), "finite")  # (all terms are positive)
+    # and of rows whose factors are infinite, by the row or by the adapter
+    a, w, down, up = _bounds_case(bz, m, pad, dtype, rank, 3)
+    a[::11, 7] = inf
+    down[1, 4, 9] = inf
+    want = _adapters_want(a, w, down, up, ids)
+    assert not bool(torch.isnan(want).any()) and bool(torch.isinf(want).any())
+    got = bz.fc_adapters(a, w, 64, down, up, ids).double()
+    far = torch.isinf(want)
+    assert bool((got[far] == want[far]).all())
+    _close(got[~far], want[~far], (HALF_STEP[dtype] + 2.0**-15) * want[~far].abs(), "finite")

@@ -147,7 +147,22 @@ __device__ __forceinline__ void put_out(const Layer& l, int64_t at, float v) {
 
 __device__ __forceinline__ float silu(float v) { return v / (1.f + expf(-v)); }
 
-// One step of K = 32 bytes of a low-rank product, added to d: what of a row's factor and of a row of `up` the lane brings
+// Eight bf16s: whether any is infinite or no number, and the same with zeros in the place of those
+__device__ __forceinline__ bool any_unbounded(const uint4& v) {
+  auto carry = [](uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; };  // an exponent of ones reaches the sign's place
+  return ((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u) != 0;
+}
+__device__ __forceinline__ uint4 bounded(const uint4& v) {
+  auto keep = [](uint32_t w) {
+    const uint32_t top = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    return w & ~(top | (top - (top >> 15)));
+  };
+  return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
+}
+
+// One step of K = 32 bytes of a low-rank product, added to d: what of a row's factor and of a row of `up` the lane brings.
+// An operand in two pieces has its infinity, or what is no number, in the first alone: times that, the second pieces of the other
+// operand, of any sign or 0, would make NaNs of infinities, and are left out.
 template <int DT>
 struct LowStep {
   uint4 hi, lo, u;
@@ -169,7 +184,9 @@ struct LowStep {
     if constexpr (DT == BZ_F32) {
       In<BZ_F32>::mma(hi, u, d);
     } else if constexpr (DT == BZ_BF16) {
-      In<BZ_BF16>::mma(lo, u, d);
+      uint4 u_some = u;
+      if (__builtin_expect(any_unbounded(u), 0)) u_some = bounded(u);
+      In<BZ_BF16>::mma(lo, u_some, d);
       In<BZ_BF16>::mma(hi, u, d);
     } else {
       // (an fp16 `up` is split the same way as the factor, so that a factor beyond fp16 does no harm)
@@ -182,9 +199,15 @@ struct LowStep {
         uh[i] = bz::fc::nearest_bf16x2(x0, x1);
         ul[i] = bz::fc::nearest_bf16x2(x0 - __uint_as_float(uh[i] << 16), x1 - __uint_as_float(uh[i] & 0xffff0000u));
       }
-      const uint4 u_hi = make_uint4(uh[0], uh[1], uh[2], uh[3]), u_lo = make_uint4(ul[0], ul[1], ul[2], ul[3]);
-      In<BZ_BF16>::mma(lo, u_hi, d);
-      In<BZ_BF16>::mma(hi, u_lo, d);
+      const uint4 u_hi = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+      uint4 u_lo = make_uint4(ul[0], ul[1], ul[2], ul[3]), u_some = u_hi, hi_some = hi;
+      if (__builtin_expect(any_unbounded(u_hi), 0)) {
+        u_some = bounded(u_hi);
+        u_lo = bounded(u_lo);  // (an infinity less itself)
+      }
+      if (__builtin_expect(any_unbounded(hi), 0)) hi_some = bounded(hi);
+      In<BZ_BF16>::mma(lo, u_some, d);
+      In<BZ_BF16>::mma(hi_some, u_lo, d);
       In<BZ_BF16>::mma(hi, u_hi, d);
     }
   }
