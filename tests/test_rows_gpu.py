@@ -1127,3 +1127,29 @@ def test_fc_adapters_of_infinite_weights(bz, m, pad, dtype, rank):
     far = torch.isinf(want)
     assert bool((got[far] == want[far]).all())
     _close(got[~far], want[~far], (HALF_STEP[dtype] + 2.0**-15) * want[~far].abs(), "finite")
+
+
+@pytest.mark.parametrize("m,pad", [(32, 0), (900, 1), (900, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [1, 5, 8, 20, 40])
+def test_fc_adapters_of_an_infinite_row_at_any_rank(bz, m, pad, dtype, rank):
+    """a row of an infinity, and one of an adapter whose scale is infinite, alone with the adapter in its block or among many rows of it, at ranks
+    that are filled up with zeros: infinite, not NaN"""
+    import torch
+    print("case", m, pad, dtype, rank, flush=True)
+    inf = float("inf")
+    a, w, down, up = _bounds_case(bz, m, pad, dtype, rank, 3)
+    a[3, 7], a[20, 0] = inf, inf
+    alone = torch.zeros(m, dtype=torch.int32, device="cuda")  # (adapter 0, and in the first block one row each of 1 and 2)
+    alone[3], alone[20] = 1, 2
+    among = torch.ones(m, dtype=torch.int32, device="cuda")
+    scale = torch.tensor([1.0, 0.5, inf], device="cuda")
+    for ids in (alone, among):
+        y = bz.fc_adapters(a, w, 64, down, up, ids, scale=scale)
+        assert bool((y[3] == inf).all()) and bool((y[20] == inf).all())
+        rest = torch.arange(m, device="cuda") % 32
+        rest = (rest != 3) & (rest != 20)
+        assert bool(torch.isfinite(y[rest]).all())
+    many = torch.full((m, ), 2, dtype=torch.int32, device="cuda")
+    y = bz.fc_adapters(a, w, 64, down, up, many, scale=scale)
+    assert bool((y == inf).all())

@@ -139,11 +139,13 @@ __global__ __launch_bounds__(kLowWaves * 64) void bz_adapters_low_kernel(Low l) 
     split.start(l.k);
     split.run(l.k, acc, (match & 0xffffu) != 0, match >> 16 != 0);
     __syncthreads();
-    split.put_sums(smem, acc, s);
+    split.put_sums(smem, acc, 1.f);
     __syncthreads();
     for (int q = tid; q < 32 * COLS; q += NT) {
       const int row = q / COLS, r = q % COLS;
-      if ((match >> row & 1) && r < ranks) put_low<DT>(l, m0 + row, r0 + r, Parts::sum(smem, row, r));
+      // (behind the rank zeros, also of a row of infinities, whose sums with zeros are no numbers; nor are an infinite scale's products with the
+      // sums of waves that have no part of K, so that it comes last)
+      if ((match >> row & 1) && r < ranks) put_low<DT>(l, m0 + row, r0 + r, r0 + r < l.rank ? s * Parts::sum(smem, row, r) : 0.f);
     }
     __syncthreads();
   }
