@@ -1153,3 +1153,20 @@ def test_fc_adapters_of_an_infinite_row_at_any_rank(bz, m, pad, dtype, rank):
     many = torch.full((m, ), 2, dtype=torch.int32, device="cuda")
     y = bz.fc_adapters(a, w, 64, down, up, many, scale=scale)
     assert bool((y == inf).all())
+
+
+@pytest.mark.parametrize("m", [20, 900])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("together", [False, True])
+def test_fc_adapters_of_the_largest_finite_factor(bz, m, dtype, together):
+    """a factor next to the largest float, which a bf16 rounds to infinity: its product with a small weight is finite"""
+    import torch
+    n, k, rank = 700, 64, 16
+    a, down, up = (torch.zeros(s, dtype=_t(dtype), device="cuda") for s in ((m, k), (m, rank, k), (m, n, rank)))
+    a[:, 0], down[:, 0, 0], up[:, :, 0] = 1.0, 1.0, 2.0**-14
+    w = torch.zeros((n, k), dtype=a.dtype, device="cuda")
+    ids = torch.zeros(m, dtype=torch.int32, device="cuda") if together else torch.arange(m, dtype=torch.int32, device="cuda")
+    for value in (3.4e38, -3.4e38, 3.3961775292304957e38, float(torch.finfo(torch.float32).max)):
+        y = bz.fc_adapters(a, w, k, down, up, ids, scale=torch.full((m, ), value, device="cuda"), out_dtype=bz.F32)
+        want = torch.full((m, n), value, dtype=torch.float32, device="cuda").double() * 2.0**-14
+        _close(y, want, 2.0**-16 * want.abs(), "%g" % value)

@@ -29,7 +29,9 @@ __device__ __forceinline__ void put_low(const Low& l, int row, int r, float v) {
   if constexpr (DT == BZ_F32) {
     ((float*)out)[r] = v;
   } else {
-    const __hip_bfloat16 hi = __float2bfloat16(v);
+    // (above the largest bf16 by less than half a step that one, not infinity)
+    const float most = 0x1.fep127f, in_reach = fabsf(v) < __builtin_huge_valf() ? fminf(fmaxf(v, -most), most) : v;
+    const __hip_bfloat16 hi = __float2bfloat16(in_reach);
     const float rest = v - __bfloat162float(hi);
     ((__hip_bfloat16*)out)[r] = hi;
     ((__hip_bfloat16*)out)[l.low_rank + r] = __float2bfloat16(fabsf(rest) < __builtin_huge_valf() ? rest : 0.f);
