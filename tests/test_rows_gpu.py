@@ -1170,3 +1170,55 @@ def test_fc_adapters_of_the_largest_finite_factor(bz, m, dtype, together):
         y = bz.fc_adapters(a, w, k, down, up, ids, scale=torch.full((m, ), value, device="cuda"), out_dtype=bz.F32)
         want = torch.full((m, n), value, dtype=torch.float32, device="cuda").double() * 2.0**-14
         _close(y, want, 2.0**-16 * want.abs(), "%g" % value)
+
+
+# ---------------------------------------------------------------------------------------------- more than 2^32 threads' worth of rows
+@pytest.mark.parametrize("rows,n", [(2**28 + 77, 2), (2**26 + 5, 129)])
+def test_route_topk_of_more_rows_than_a_launch_has_threads_for(bz, rows, n):
+    import torch
+    logits = torch.empty((rows, n), dtype=torch.float16, device="cuda").normal_()
+    ids, w = bz.route_topk(logits, 1, renormalize=True)
+    assert bool((w == 1).all())
+    for at in (0, rows // 2 - 500, 2**25 - 500, 2**27 - 500, rows - 1000):
+        part = logits[at:at + 1000].float()
+        if part.shape[0]:
+            first = (part == part.amax(1, keepdim=True)).int().argmax(1)
+            assert torch.equal(ids[at:at + part.shape[0], 0].long(), first), at
+    del logits, ids, w
+    torch.cuda.empty_cache()
+
+
+def test_merge_gradient_of_more_rows_than_a_launch_has_threads_for(bz):
+    import torch
+    rows, dim = 2**26 + 3, 8
+    dy, xs = (torch.empty((rows, dim), dtype=torch.float16, device="cuda").normal_() for _ in range(2))
+    position = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    w = torch.empty((rows, 1), device="cuda").normal_()
+    dxs, dw = bz.merge_rows_grad(dy, xs, position, w, dxs=torch.empty_like(xs))
+    for at in (0, 2**25 - 500, rows - 1000):
+        t = slice(at, at + 1000)
+        to = position[t, 0].long()
+        want = (w[t].double() * dy[t].double())
+        _close(dxs[to], want, (HALF_STEP["f16"] + EPS) * want.abs() * (1 + 2.0**-8) + 2.0**-25, "dxs from %d" % at)
+        products = dy[t].double() * xs[to].double()
+        _close(dw[t, 0], products.sum(1), (dim + 4) * EPS * products.abs().sum(1), "dweights from %d" % at)
+    del dy, xs, dxs, dw, w, position
+    torch.cuda.empty_cache()
+
+
+def test_rows_of_more_chunks_than_a_launch_has_threads_move_and_merge(bz):
+    import torch
+    rows, dim = 2**22 + 1, 8 * 1025
+    few = _normal(0, (100, dim), 1.0, "f16")
+    position = torch.randint(100, (rows, 1), device="cuda", dtype=torch.int32)
+    x = bz.merge_rows(few, position)
+    ats = [slice(0, 300), slice(2**31 // 1025 - 100, 2**31 // 1025 + 100), slice(rows - 300, rows)]
+    for t in ats:
+        assert torch.equal(x[t], few[position[t, 0].long()])
+    ids = (torch.arange(rows, device="cuda") % 2).to(torch.int32)[:, None].contiguous()
+    offsets, order, to, xs = bz.group_rows(ids, 2, x=x)
+    assert offsets.tolist() == [0, rows // 2 + 1, rows]
+    for t in ats:
+        assert torch.equal(xs[to[t, 0].long()], x[t])
+    del x, xs
+    torch.cuda.empty_cache()

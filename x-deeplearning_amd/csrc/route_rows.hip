@@ -109,13 +109,27 @@ __global__ __launch_bounds__(256) void bz_route_kernel(const char* __restrict__ 
   }
 }
 
+// A launch has fewer than 2^32 threads: more rows, of `threads` each, go by in parts.  f(first row, rows of the part)
+constexpr int64_t kPartThreads = (int64_t)1 << 31;
+template <typename F>
+int in_parts(int64_t rows, int64_t threads, const F& f) {
+  const int64_t part = std::max<int64_t>(1, kPartThreads / threads);
+  for (int64_t r = 0; r < rows; r += part) {
+    const int rc = f(r, std::min(part, rows - r));
+    if (rc != BZ_OK) return rc;
+  }
+  return BZ_OK;
+}
+
 template <int DT, int L, int V>
 int launch_route(const bz_route_desc& d, hipStream_t st) {
-  const int64_t wg = (d.rows * L + 255) / 256;
-  hipLaunchKernelGGL((bz_route_kernel<DT, L, V>), dim3((uint32_t)wg), dim3(256), 0, st, (const char*)d.logits, d.ld, d.rows, d.n, d.k,
-                     d.ids, d.weights, d.score, d.renormalize, d.scale);
-  BZ_LAUNCH_OK("bz_route_kernel");
-  return BZ_OK;
+  return in_parts(d.rows, L, [&](int64_t r0, int64_t rows) {
+    hipLaunchKernelGGL((bz_route_kernel<DT, L, V>), dim3((uint32_t)((rows * L + 255) / 256)), dim3(256), 0, st,
+                       (const char*)d.logits + r0 * d.ld * Elem<DT>::kSize, d.ld, rows, d.n, d.k, d.ids + r0 * d.k, d.weights + r0 * d.k, d.score,
+                       d.renormalize, d.scale);
+    BZ_LAUNCH_OK("bz_route_kernel");
+    return (int)BZ_OK;
+  });
 }
 
 template <int DT>
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(kGroupThreads) void bz_group_few_kernel(const int32
   __shared__ int to[kFewRun];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int begin = blockIdx.x * run, end = min(begin + run, n);
-  const uint32_t chunks = (uint32_t)(dim + CH - 1) / CH, items = (uint32_t)(end - begin) / (uint32_t)per * chunks;
+  const uint32_t chunks = (uint32_t)(dim - 1) / CH + 1, items = (uint32_t)(end - begin) / (uint32_t)per * chunks;
   const int64_t row0 = (uint32_t)begin / (uint32_t)per;
   auto load = [&](uint32_t q) {
     const uint32_t row = q / chunks;
@@ -463,7 +477,7 @@ __global__ __launch_bounds__(256) void bz_merge_grad_kernel(const char* __restri
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int lane = threadIdx.x & 63;
-  const int chunks = (dim + CH - 1) / CH;
+  const int chunks = (dim - 1) / CH + 1;
   int at[K];
   float w[K], dot[K];
 #pragma unroll
@@ -518,8 +532,6 @@ int by_type(int dt, const F& f) {
   if (dt == BZ_F16) return f(std::integral_constant<int, BZ_F16>());
   return f(std::integral_constant<int, BZ_BF16>());
 }
-
-constexpr int64_t kMaxWorkgroups = 0x7fffffff;
 
 // Whether rows that are written are more than the 256 MB cache keeps for whoever reads them next.  Written past the caches they take a tenth
 // less (16384 x 8 rows of 2048 bf16 moved in 115 us, 128 with ordinary stores; the gradient of 8192 x 8 such rows 134 and 144), but what
@@ -583,7 +595,7 @@ int bz_group_rows(const bz_group_desc* desc, bz_stream_t stream) {
   while (d.groups >> bits) ++bits;  // (the number `groups`, of entries in none, among them)
   int32_t* counts = need > 0 ? (int32_t*)d.scratch : nullptr;
   const int64_t few = (std::max<int64_t>(1, d.n / 512) + d.per - 1) / std::max(1, d.per) * d.per;  // about 512 workgroups, whole rows each
-  if (d.x != nullptr && d.n > 0 && d.n <= kFewEntries && d.n / d.per <= kFewRows && few <= kFewRun)
+  if (d.x != nullptr && d.n > 0 && d.n <= kFewEntries && d.n / d.per <= kFewRows && few <= kFewRun && d.dim < 1 << 24)  // (its chunks of 32 bits)
     return by_type(d.dtype, [&](auto dt) {
       hipLaunchKernelGGL((bz_group_few_kernel<decltype(dt)::value>), dim3((uint32_t)((d.n + few - 1) / few)), dim3(kGroupThreads), 0, st, d.ids,
                          (int)d.n, (int)few, d.groups, bits, d.offsets, d.order, d.position, (const char*)d.x, (char*)d.xs, d.ld_x, d.ld_xs,
@@ -603,14 +615,16 @@ int bz_group_rows(const bz_group_desc* desc, bz_stream_t stream) {
   if (d.x == nullptr || d.n == 0) return BZ_OK;
   return by_type(d.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    const int chunks = (d.dim + 16 / Elem<DT>::kSize - 1) / (16 / Elem<DT>::kSize);
-    const int64_t items = d.n / d.per * chunks, blocks = (items + 255) / 256;
-    BZ_REQUIRE(blocks <= kMaxWorkgroups, "bz_group_rows: too many elements");
-    auto* kernel = beyond_caches(d.n * d.dim * Elem<DT>::kSize) ? bz_spread_kernel<DT, true> : bz_spread_kernel<DT, false>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(256), 0, st, (const char*)d.x, (const int32_t*)d.position,
-                       (char*)d.xs, items, d.ld_x, d.ld_xs, chunks, d.dim, d.per);
-    BZ_LAUNCH_OK("bz_spread_kernel");
-    return (int)BZ_OK;
+    const int chunks = (d.dim - 1) / (16 / Elem<DT>::kSize) + 1;
+    constexpr int ES = Elem<DT>::kSize;
+    auto* kernel = beyond_caches(d.n * d.dim * ES) ? bz_spread_kernel<DT, true> : bz_spread_kernel<DT, false>;
+    return in_parts(d.n / d.per, chunks, [&](int64_t r0, int64_t rows) {
+      const int64_t items = rows * chunks;
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)((items + 255) / 256)), dim3(256), 0, st, (const char*)d.x + r0 * d.ld_x * ES,
+                         (const int32_t*)d.position + r0 * d.per, (char*)d.xs, items, d.ld_x, d.ld_xs, chunks, d.dim, d.per);
+      BZ_LAUNCH_OK("bz_spread_kernel");
+      return (int)BZ_OK;
+    });
   });
 }
 
@@ -628,17 +642,19 @@ int bz_merge_rows(const bz_merge_desc* desc, bz_stream_t stream) {
   BZ_REQUIRE((d.xs || d.n == 0) && d.position && d.y, "bz_merge_rows: null pointer");
   return by_type(d.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    const int chunks = (d.dim + 16 / Elem<DT>::kSize - 1) / (16 / Elem<DT>::kSize);
-    const int64_t items = d.rows * chunks, blocks = (items + 255) / 256;
-    BZ_REQUIRE(blocks <= kMaxWorkgroups, "bz_merge_rows: too many elements");
+    const int chunks = (d.dim - 1) / (16 / Elem<DT>::kSize) + 1;
     auto launch = [&](auto* y) {
       using OutT = std::remove_pointer_t<decltype(y)>;
       auto* kernel = d.k <= 2 ? bz_merge_kernel<DT, OutT, 2> : d.k <= 4 ? bz_merge_kernel<DT, OutT, 4> : d.k <= 8 ? bz_merge_kernel<DT, OutT, 8>
                                                                                                                   : bz_merge_kernel<DT, OutT, 16>;
-      hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(256), 0, bz::as_stream(stream), (const char*)d.xs,
-                         d.position, d.weights, y, items, d.n, d.ld_xs, d.ld_y, chunks, d.dim, d.k);
-      BZ_LAUNCH_OK("bz_merge_kernel");
-      return (int)BZ_OK;
+      return in_parts(d.rows, chunks, [&](int64_t r0, int64_t rows) {
+        const int64_t items = rows * chunks;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)((items + 255) / 256)), dim3(256), 0, bz::as_stream(stream), (const char*)d.xs,
+                           d.position + r0 * d.k, d.weights != nullptr ? d.weights + r0 * d.k : nullptr, y + r0 * d.ld_y, items, d.n, d.ld_xs, d.ld_y,
+                           chunks, d.dim, d.k);
+        BZ_LAUNCH_OK("bz_merge_kernel");
+        return (int)BZ_OK;
+      });
     };
     return d.out_dtype == DT ? launch((typename Elem<DT>::type*)d.y) : launch((float*)d.y);
   });
@@ -666,10 +682,14 @@ int bz_merge_rows_grad(const bz_merge_grad_desc* desc, bz_stream_t stream) {
     };
     const int64_t bytes = d.dxs ? std::min<int64_t>(d.rows * d.k, d.n) * d.dim * Elem<DT>::kSize : 0;
     auto* kernel = beyond_caches(bytes) ? pick(std::true_type()) : pick(std::false_type());
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((d.rows + 3) / 4)), dim3(256), 0, bz::as_stream(stream), (const char*)d.dy, (const char*)d.xs,
-                       d.position, d.weights, (char*)d.dxs, d.dweights, d.rows, d.n, d.ld_dy, d.ld_xs, d.ld_dxs, d.k, d.dim);
-    BZ_LAUNCH_OK("bz_merge_grad_kernel");
-    return (int)BZ_OK;
+    return in_parts(d.rows, 64, [&](int64_t r0, int64_t rows) {
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, bz::as_stream(stream),
+                         (const char*)d.dy + r0 * d.ld_dy * Elem<DT>::kSize, (const char*)d.xs, d.position + r0 * d.k,
+                         d.weights != nullptr ? d.weights + r0 * d.k : nullptr, (char*)d.dxs, d.dweights != nullptr ? d.dweights + r0 * d.k : nullptr,
+                         rows, d.n, d.ld_dy, d.ld_xs, d.ld_dxs, d.k, d.dim);
+      BZ_LAUNCH_OK("bz_merge_grad_kernel");
+      return (int)BZ_OK;
+    });
   });
 }
 
