@@ -690,6 +690,8 @@ BZ_API int bz_merge_rows_grad(const bz_merge_grad_desc* desc, bz_stream_t stream
  * act: any bz_act but the softmax, its parameters [groups, act_size] (PRelu, 1 or n) or [groups, n] (Dice, act_size n or 0); or BZ_ACT_SWIGLU:
  * w[g] is [2 * n, ldw] and bias [groups, 2 * n], and with v = a * w[g]^T + bias[g]
  *   y[r, c] = v[c] / (1 + e^-v[c]) * v[n + c]
+ * A layer that would take a launch of 2^32 threads and more is refused, here and in bz_fc_adapters: 2^36 outputs (2^40 of aligned
+ * 2-byte operands within 4 GB), some 2^30 rows, or some 2^28 columns of few rows.
  * BZ_ACT_SIGMOID is 1 / (1 + e^-v) here and in bz_fc_adapters, so that it has a value for any v, and BZ_ACT_LEAKY_RELU with act_alpha 0 is 0 for
  * any v below 0.
  */

@@ -141,3 +141,24 @@ def test_the_binding_refuses_dice_of_one_parameter_a_group(bz):
         assert bz._act_fields("grouped_fc", bz.ACT_PRELU, (one, ), 8, groups, -1)[1] == 1
         with pytest.raises(bz.BlazeHipError, match="act_params"):
             bz._act_fields("grouped_fc", bz.ACT_PRELU, (full, one), 8, groups, -1)
+
+
+def test_layers_beyond_a_launch_are_refused_before_anything_is_launched(bz):
+    """a launch has fewer than 2^32 threads: what would take more is an argument that does not fit, not a launch that fails"""
+    layer = dict(a=P, w=P, y=P, in_dtype=bz.F16, out_dtype=bz.F16, k=16, lda=16, ldw=16, act=bz.ACT_NONE)
+    sizes = [dict(m=2**31 - 1, n=64, ldy=64), dict(m=2**30, n=64, ldy=64), dict(m=32, n=2**31 - 64, ldy=2**31), dict(m=48, n=2**28, ldy=2**28),
+             dict(m=2**20, n=2**17, ldy=2**17), dict(m=2**20, n=2**17, ldy=2**17, in_dtype=bz.F32, out_dtype=bz.F32)]
+    for size in sizes:
+        # (aligned 2-byte operands within 4 GB have tiles of 256 x 256: 2^37 outputs are 2^21 of them, 2^29 threads, which a launch may have)
+        for pitch in (17, ) if size is sizes[4] else (16, 17):
+            good = dict(layer, **size)
+            good.update(lda=pitch, ldw=pitch)
+            rc, text = _rc(bz, "bz_grouped_fc", _fill(bz.GroupedFcDesc, offsets=P, groups=1, a_count=size["m"], **good))
+            assert rc == bz.EINVAL and "bz_grouped_fc" in text and "too many" in text, (size, rc, text)
+            for adapters in (0, 3):
+                rc, text = _rc(bz, "bz_fc_adapters", _fill(bz.FcAdaptersDesc, down=P, up=P, ids=P, scratch=P, scratch_bytes=2**50, ld_down=16, ld_up=8, rank=8,
+                                                           adapters=adapters, down_stride=128, up_stride=2**40, alpha=1.0, beta=1.0, **good))
+                assert rc == bz.EINVAL and "bz_fc_adapters" in text and "too many" in text, (size, adapters, rc, text)
+    gated = dict(layer, m=48, n=2**27, ldy=2**27, act=bz.ACT_SWIGLU)
+    rc, text = _rc(bz, "bz_grouped_fc", _fill(bz.GroupedFcDesc, offsets=P, groups=1, a_count=48, **gated))
+    assert rc == bz.EINVAL and "too many" in text

@@ -155,8 +155,6 @@ __global__ __launch_bounds__(kLowWaves * 64) void bz_adapters_low_kernel(Low l) 
 
 template <int DT>
 int run_low(const bz_fc_adapters_desc& d, int low_rank, hipStream_t st) {
-  const Low l = {(const char*)d.a, (const char*)d.down, d.ids, d.scale, (char*)d.scratch, d.lda, d.ld_down, d.down_stride, d.m, d.k,
-                 d.adapters, d.rank, low_rank};
   constexpr int ES = In<DT>::kSize;
   const bool aligned = (uintptr_t)d.a % 16 == 0 && (uintptr_t)d.down % 16 == 0 && d.lda * ES % 16 == 0 && d.ld_down * ES % 16 == 0 &&
                        d.down_stride * ES % 16 == 0 && (int64_t)d.k * ES % 16 == 0;
@@ -167,10 +165,15 @@ int run_low(const bz_fc_adapters_desc& d, int low_rank, hipStream_t st) {
     static Lds lds;
     const int rc = lds.allow((const void*)kernel, LDS);
     if (rc != BZ_OK) return rc;
-    const int blocks = (d.m + 31) / 32, parts = (low_rank + COLS - 1) / COLS;
-    const int turns = std::max(1, std::min(32, 512 / std::min(512, blocks * parts)));
-    hipLaunchKernelGGL(kernel, dim3(blocks, parts, turns), dim3(kLowWaves * 64), LDS, st, l);
-    BZ_LAUNCH_OK("bz_adapters_low_kernel");
+    constexpr int64_t kPart = 1 << 26;  // rows of a launch, which has fewer than 2^32 threads
+    for (int64_t r0 = 0; r0 < d.m; r0 += kPart) {
+      const int m = (int)std::min<int64_t>(kPart, d.m - r0), blocks = (m + 31) / 32, parts = (low_rank + COLS - 1) / COLS;
+      const Low l = {(const char*)d.a + r0 * d.lda * ES, (const char*)d.down, d.ids + r0, d.scale, (char*)d.scratch + r0 * low_rank * 4, d.lda, d.ld_down,
+                     d.down_stride, m, d.k, d.adapters, d.rank, low_rank};
+      const int turns = std::max(1, std::min(32, 512 / std::min(512, blocks * parts)));
+      hipLaunchKernelGGL(kernel, dim3(blocks, parts, turns), dim3(kLowWaves * 64), LDS, st, l);
+      BZ_LAUNCH_OK("bz_adapters_low_kernel");
+    }
     return (int)BZ_OK;
   };
   auto by_rank = [&](auto aligned_c) {
@@ -180,8 +183,11 @@ int run_low(const bz_fc_adapters_desc& d, int low_rank, hipStream_t st) {
 }
 
 template <int DT>
-int run(const Layer& l, hipStream_t st) {
-  return l.adapters > 0 ? run_layer<DT, false, true>(l, st) : run_layer<DT, false, false>(l, st);
+int run(const Layer& l, const Call& call) {
+  return l.adapters > 0 ? run_layer<DT, false, true>(l, call) : run_layer<DT, false, false>(l, call);
+}
+int run(int dtype, const Layer& l, const Call& call) {
+  return dtype == BZ_F32 ? run<BZ_F32>(l, call) : dtype == BZ_F16 ? run<BZ_F16>(l, call) : run<BZ_BF16>(l, call);
 }
 
 int low_rank_of(int rank) { return (rank + 15) / 16 * 16; }
@@ -245,6 +251,7 @@ int bz_fc_adapters(const bz_fc_adapters_desc* desc, bz_stream_t stream) {
   l.ep.beta = d.beta;
   l.ep.act_alpha = d.act_alpha;
   l.adapters = d.adapters;
+  l.out_f32 = d.out_dtype == BZ_F32;
   const hipStream_t st = bz::as_stream(stream);
   if (d.adapters > 0) {
     l.rank = d.rank;
@@ -254,14 +261,16 @@ int bz_fc_adapters(const bz_fc_adapters_desc* desc, bz_stream_t stream) {
     l.up = (const char*)d.up;
     l.ld_up = d.ld_up;
     l.up_stride = d.up_stride;
+    // what can be refused is refused before the factors are launched (no kernel has more than a thread an output, 32 by 16 of them whole)
+    if (((int64_t)d.m + 31) * ((int64_t)d.n + 15) >= (int64_t)1 << 31) {
+      const int rc = run(d.in_dtype, l, {"bz_fc_adapters", st, true});
+      if (rc != BZ_OK) return rc;
+    }
     const int done = d.in_dtype == BZ_F32 ? run_low<BZ_F32>(d, l.low_rank, st)
                      : d.in_dtype == BZ_F16 ? run_low<BZ_F16>(d, l.low_rank, st) : run_low<BZ_BF16>(d, l.low_rank, st);
     if (done != BZ_OK) return done;
   }
-  l.out_f32 = d.out_dtype == BZ_F32;
-  if (d.in_dtype == BZ_F32) return run<BZ_F32>(l, st);
-  if (d.in_dtype == BZ_F16) return run<BZ_F16>(l, st);
-  return run<BZ_BF16>(l, st);
+  return run(d.in_dtype, l, {"bz_fc_adapters", st});
 }
 
 }  // extern "C"

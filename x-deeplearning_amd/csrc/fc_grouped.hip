@@ -7,7 +7,8 @@ using namespace bz::groups;
 
 template <int DT>
 int run(const Layer& l, bool gated, hipStream_t st) {
-  return gated ? run_layer<DT, true, false>(l, st) : run_layer<DT, false, false>(l, st);
+  const Call call = {"bz_grouped_fc", st};
+  return gated ? run_layer<DT, true, false>(l, call) : run_layer<DT, false, false>(l, call);
 }
 
 }  // namespace

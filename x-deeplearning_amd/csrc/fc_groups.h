@@ -123,6 +123,15 @@ __device__ __forceinline__ int count_tiles(const Layer& l) {
   }
   return __builtin_amdgcn_readfirstlane(bz::rows::reduce<64>(tiles, [](int a, int b) { return a + b; }));
 }
+// Who asks for a layer, and where; check_only: whether it can be launched, and no more
+struct Call {
+  const char* who;
+  hipStream_t stream;
+  bool check_only = false;
+};
+// (a launch has fewer than 2^32 threads)
+constexpr const char* kTooManyTiles = "%s: %lld tiles of %d rows and %d columns are too many for a launch";
+
 // how many tiles there can be
 inline int64_t most_tiles(int64_t m, int groups, int bm) { return m / bm + std::min<int64_t>(groups, m); }
 
@@ -459,11 +468,12 @@ __global__ __launch_bounds__(256) void bz_groups_tile_kernel(Layer l, int tiles_
 }
 
 template <int DT, int BM, int BN, bool GATED, bool ADAPTERS>
-int launch_tile(const Layer& l, hipStream_t st) {
+int launch_tile(const Layer& l, const Call& call) {
   const int bn = GATED ? BN / 2 : BN;
   const int64_t tiles_n = (l.n + bn - 1) / bn, tiles = most_tiles(l.m, l.offsets ? l.groups : 1, BM) * tiles_n;
-  BZ_REQUIRE(tiles < (int64_t)1 << 31, "too many tiles");
-  hipLaunchKernelGGL((bz_groups_tile_kernel<DT, BM, BN, GATED, ADAPTERS>), dim3((uint32_t)tiles), dim3(256), 0, st, l, (int)tiles_n);
+  BZ_REQUIRE(tiles * 256 < (int64_t)1 << 32, kTooManyTiles, call.who, (long long)tiles, l.m, l.n);
+  if (call.check_only) return BZ_OK;
+  hipLaunchKernelGGL((bz_groups_tile_kernel<DT, BM, BN, GATED, ADAPTERS>), dim3((uint32_t)tiles), dim3(256), 0, call.stream, l, (int)tiles_n);
   BZ_LAUNCH_OK("bz_groups_tile_kernel");
   return BZ_OK;
 }
@@ -718,10 +728,11 @@ struct Lds {
 };
 
 template <int DT, int NW, bool ALIGNED, bool GATED, bool ADAPTERS, int COLS = 32>
-int launch_split(const Layer& l, hipStream_t st) {
+int launch_split(const Layer& l, const Call& call) {
   const int bn = GATED ? 16 : COLS;
   const int64_t tiles_n = (l.n + bn - 1) / bn, tiles = most_tiles(l.m, l.offsets ? l.groups : 1, 32) * tiles_n;
-  BZ_REQUIRE(tiles < (int64_t)1 << 31, "too many tiles");
+  BZ_REQUIRE(tiles * (NW * 64) < (int64_t)1 << 32, kTooManyTiles, call.who, (long long)tiles, l.m, l.n);
+  if (call.check_only) return BZ_OK;
   constexpr int LDS = Split<DT, NW, ALIGNED, COLS>::LDS;
   auto* kernel = bz_groups_split_kernel<DT, NW, ALIGNED, GATED, ADAPTERS, COLS>;
   if constexpr (LDS > 64 << 10) {
@@ -729,7 +740,7 @@ int launch_split(const Layer& l, hipStream_t st) {
     const int rc = lds.allow((const void*)kernel, LDS);
     if (rc != BZ_OK) return rc;
   }
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)tiles), dim3(NW * 64), LDS, st, l, (int)tiles_n);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)tiles), dim3(NW * 64), LDS, call.stream, l, (int)tiles_n);
   BZ_LAUNCH_OK("bz_groups_split_kernel");
   return BZ_OK;
 }
@@ -1294,10 +1305,11 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
 }
 
 template <int DT, int TM, int TN, int S, bool GATED, bool ADAPTERS>
-int launch_wide(const Layer& l, hipStream_t st) {
+int launch_wide(const Layer& l, const Call& call) {
   const int bm = 64 * TM, bn = GATED ? 32 * TN : 64 * TN;
   const int64_t tiles_n = (l.n + bn - 1) / bn, tiles = most_tiles(l.m, l.offsets ? l.groups : 1, bm) * tiles_n;
-  BZ_REQUIRE(tiles < (int64_t)1 << 30, "too many tiles");
+  BZ_REQUIRE((tiles + 7) * 256 < (int64_t)1 << 32, kTooManyTiles, call.who, (long long)tiles, l.m, l.n);
+  if (call.check_only) return BZ_OK;
   constexpr int LDS = S * 64 * (TM + TN) * 128 + (4 * 64 * TN + 64 * TM) * 4;
   auto* kernel = bz_groups_wide_kernel<DT, TM, TN, S, GATED, ADAPTERS>;
   if constexpr (LDS > 64 << 10) {
@@ -1305,7 +1317,7 @@ int launch_wide(const Layer& l, hipStream_t st) {
     const int rc = lds.allow((const void*)kernel, LDS);
     if (rc != BZ_OK) return rc;
   }
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(256), LDS, st, l, (int)tiles_n);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(256), LDS, call.stream, l, (int)tiles_n);
   BZ_LAUNCH_OK("bz_groups_wide_kernel");
   return BZ_OK;
 }
@@ -1345,7 +1357,7 @@ inline int64_t wide_cost(int64_t tiles, const int (&part)[AT_ONCE]) {
 // What is not aligned: the tile kernel, which needs no alignment (where not the few rows' one: 1023x1023, 500 rows 11.6 by that and 16.7 by
 // tiles, fp32 700 rows 54.7 and 49.6, with adapters fp16 300 rows 24.7 and 24.2).
 template <int DT, bool GATED, bool ADAPTERS>
-int run_layer(const Layer& l, hipStream_t st) {
+int run_layer(const Layer& l, const Call& call) {
   const int groups = l.offsets ? l.groups : 1;
   const bool aligned = rows_aligned(l, In<DT>::kSize);
   const int64_t limit = (int64_t)1 << 32, es = In<DT>::kSize;
@@ -1357,11 +1369,11 @@ int run_layer(const Layer& l, hipStream_t st) {
   if (l.m <= 48 * (int64_t)groups || small <= (!aligned ? (ADAPTERS ? 256 : 512) : DT == BZ_F32 ? 768 : 512)) {
     if constexpr (!GATED)
       if (small <= 128)
-        return aligned ? launch_split<DT, 8, true, false, ADAPTERS, 16>(l, st) : launch_split<DT, 8, false, false, ADAPTERS, 16>(l, st);
-    if (!aligned) return launch_split<DT, 4, false, GATED, ADAPTERS>(l, st);
+        return aligned ? launch_split<DT, 8, true, false, ADAPTERS, 16>(l, call) : launch_split<DT, 8, false, false, ADAPTERS, 16>(l, call);
+    if (!aligned) return launch_split<DT, 4, false, GATED, ADAPTERS>(l, call);
     if constexpr (!ADAPTERS)
-      if (small > 256) return launch_split<DT, 4, true, GATED, ADAPTERS>(l, st);
-    return launch_split<DT, 8, true, GATED, ADAPTERS>(l, st);
+      if (small > 256) return launch_split<DT, 4, true, GATED, ADAPTERS>(l, call);
+    return launch_split<DT, 8, true, GATED, ADAPTERS>(l, call);
   }
   if (aligned && near) {
     if constexpr (DT != BZ_F32) {
@@ -1369,13 +1381,13 @@ int run_layer(const Layer& l, hipStream_t st) {
       const int64_t c12 = wide_cost<2>(tiles(64, 128 / G), {26, 33});
       const int64_t c11 = wide_cost<3>(tiles(64, 64), {19, 25, 31});
       const int64_t large = std::min(std::min(c44, c22), c12), least = GATED ? large : std::min(large, c11);
-      if (c44 == least) return launch_wide<DT, 4, 4, 2, GATED, ADAPTERS>(l, st);
-      if (c12 == least) return launch_wide<DT, 1, 2, 3, GATED, ADAPTERS>(l, st);
-      if (c22 == least) return launch_wide<DT, 2, 2, 2, GATED, ADAPTERS>(l, st);
+      if (c44 == least) return launch_wide<DT, 4, 4, 2, GATED, ADAPTERS>(l, call);
+      if (c12 == least) return launch_wide<DT, 1, 2, 3, GATED, ADAPTERS>(l, call);
+      if (c22 == least) return launch_wide<DT, 2, 2, 2, GATED, ADAPTERS>(l, call);
     }
-    return launch_wide<DT, 1, GATED ? 2 : 1, 3, GATED, ADAPTERS>(l, st);
+    return launch_wide<DT, 1, GATED ? 2 : 1, 3, GATED, ADAPTERS>(l, call);
   }
-  return launch_tile<DT, 64, GATED ? 128 : 64, GATED, ADAPTERS>(l, st);
+  return launch_tile<DT, 64, GATED ? 128 : 64, GATED, ADAPTERS>(l, call);
 }
 
 }  // namespace groups
