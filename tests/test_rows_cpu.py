@@ -162,3 +162,54 @@ def test_layers_beyond_a_launch_are_refused_before_anything_is_launched(bz):
     gated = dict(layer, m=48, n=2**27, ldy=2**27, act=bz.ACT_SWIGLU)
     rc, text = _rc(bz, "bz_grouped_fc", _fill(bz.GroupedFcDesc, offsets=P, groups=1, a_count=48, **gated))
     assert rc == bz.EINVAL and "too many" in text
+
+
+def test_tiles_of_offsets_that_run_backwards_stay_in_the_grid(tmp_path):
+    """Offsets that go back and forth count a layer's rows up to 512 times, whose tiles times those of its columns pass 32 bits where the layer's
+    own do not.  The kernel for many rows counts no further than its launch goes, and with such a count a workgroup has a tile of the grid or none,
+    and every tile is one workgroup's."""
+    import shutil
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc")
+    src, exe = tmp_path / "tiles.hip", str(tmp_path / "tiles")
+    src.write_text(r"""
+#include <stdio.h>
+#include <vector>
+#include "fc_groups.h"
+int bz::fail(int code, const char*, ...) { return code; }
+using namespace bz::groups;
+int main() {
+  for (int64_t m : {1, 63, 64, 1000, 1 << 17, 1 << 20})
+    for (int groups : {1, 3, 1024})
+      for (int tiles_n : {1, 7, 2048, 16384}) {
+        const int64_t most = most_tiles(m, groups, 64);
+        if ((most * tiles_n + 7) * 256 >= (int64_t)1 << 32) continue;  // (refused on the host)
+        if (64 * most >= (int64_t)1 << 31) return 4;  // (what the lanes have counted between them)
+        for (int64_t counted : {most, most - 1, most / 2, 512 * (m / 64 + 1)}) {
+          const int tiles_m = (int)(counted < most ? counted : most);
+          const uint32_t blocks = (uint32_t)((most * tiles_n + 7) / 8 * 8), step = blocks > 1000000 ? 997 : 1;
+          std::vector<char> seen(step == 1 && tiles_m > 0 ? (size_t)tiles_m * tiles_n : 0);
+          for (uint32_t b = 0; b < blocks; b += step) {
+            int tm = -1, tn = -1;
+            if (!wide_tile(tiles_m, tiles_n, b, tm, tn)) continue;
+            if (tm < 0 || tm >= tiles_m || tn < 0 || tn >= tiles_n) {
+              printf("m %lld, %d groups, %d tiles of columns, %lld counted: workgroup %u has tile %d, %d\n", (long long)m, groups, tiles_n, (long long)counted, b, tm, tn);
+              return 1;
+            }
+            if (step == 1 && seen[(size_t)tm * tiles_n + tn]++) return 2;
+          }
+          for (char c : seen)
+            if (c != 1) return 3;
+        }
+      }
+  return 0;
+}
+""")
+    csrc = os.path.join(ROOT, "x-deeplearning_amd", "csrc")
+    subprocess.run([hipcc, "--offload-arch=gfx950", "--cuda-host-only", "-std=c++17", "-O1", "-I" + os.path.join(ROOT, "include"), "-I" + csrc, str(src), "-o", exe],
+                   check=True, capture_output=True, timeout=300)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, (r.returncode, r.stdout)
+    # and the kernel counts no further
+    assert "reduce<64>(min(tiles, most), [](int a, int b) { return a + b; }), most)" in open(os.path.join(csrc, "fc_groups.h")).read()

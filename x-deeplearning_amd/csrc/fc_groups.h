@@ -110,18 +110,21 @@ __device__ __forceinline__ bool find_tile(const Layer& l, int tile, int& group, 
   }
   return false;
 }
-// The number of tiles of BM rows that all groups have together
+// how many tiles of bm rows there can be
+__host__ __device__ inline int64_t most_tiles(int64_t m, int groups, int bm) { return m / bm + (groups < m ? groups : m); }
+// The number of tiles of BM rows that all groups have together.  Offsets that run backwards count rows again and again: no more tiles than a
+// launch is made for (64 times as many fit 32 bits: it has a workgroup of 256 threads for each).
 template <int BM>
 __device__ __forceinline__ int count_tiles(const Layer& l) {
   if (l.offsets == nullptr) return (l.m + BM - 1) / BM;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, most = (int)most_tiles(l.m, l.groups, BM);
   int tiles = 0;
   for (int g = lane; g < l.groups; g += 64) {
     int begin, end;
     group_range(l.offsets, g, l.m, begin, end);
     tiles += (end - begin + BM - 1) / BM;
   }
-  return __builtin_amdgcn_readfirstlane(bz::rows::reduce<64>(tiles, [](int a, int b) { return a + b; }));
+  return __builtin_amdgcn_readfirstlane(min(bz::rows::reduce<64>(min(tiles, most), [](int a, int b) { return a + b; }), most));
 }
 // Who asks for a layer, and where; check_only: whether it can be launched, and no more
 struct Call {
@@ -132,8 +135,6 @@ struct Call {
 // (a launch has fewer than 2^32 threads)
 constexpr const char* kTooManyTiles = "%s: %lld tiles of %d rows and %d columns are too many for a launch";
 
-// how many tiles there can be
-inline int64_t most_tiles(int64_t m, int groups, int bm) { return m / bm + std::min<int64_t>(groups, m); }
 
 // address of row r's input, null for a row of zeros
 __device__ __forceinline__ const char* input_row(const Layer& l, int r, int es) {
@@ -765,6 +766,19 @@ int launch_split(const Layer& l, const Call& call) {
 // experts, 8192 rows x 4, 2048 -> 1024: 339 us, 811 TFLOP/s; what is missing are tiles that groups do not fill, the last round of
 // workgroups and the starts and ends of tiles, which nothing covers.
 constexpr int kWideBand = 8;
+// which tile of tiles_m x tiles_n (their product and 8 more below 2^31) workgroup `block` has; false: none
+__host__ __device__ inline bool wide_tile(int tiles_m, int tiles_n, uint32_t block, int& tile_m, int& tile_n) {
+  const int each = (tiles_m * tiles_n + 7) / 8;
+  int t = (int)(block >> 3);
+  if (t >= each) return false;
+  t += (int)(block & 7) * each;
+  if (t >= tiles_m * tiles_n) return false;
+  const int band = t / (kWideBand * tiles_n), in_band = t - band * (kWideBand * tiles_n), left = tiles_m - band * kWideBand;
+  const int high = left < kWideBand ? left : kWideBand;
+  tile_n = in_band / high;
+  tile_m = band * kWideBand + in_band % high;
+  return true;
+}
 // The loads are free to move among reads of LDS: only the waits and barriers keep them apart.
 __device__ __forceinline__ void lds_load_free(const char* g, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_addr) : "m0");
@@ -845,15 +859,9 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
   static_assert(!GATED || TN % 2 == 0, "a wave has both of a column's");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
-  const int tiles_m = count_tiles<BM>(l), each = (tiles_m * tiles_n + 7) / 8;
-  int t = (int)(blockIdx.x >> 3);
-  if (t >= each) return;
-  t += (int)(blockIdx.x & 7) * each;
-  if (t >= tiles_m * tiles_n) return;
-  const int band = t / (kWideBand * tiles_n), in_band = t - band * (kWideBand * tiles_n), high = min(kWideBand, tiles_m - band * kWideBand);
-  const int tile_n = in_band / high;
-  int group, m0, m1;
-  if (!find_tile<BM>(l, band * kWideBand + in_band % high, group, m0, m1)) return;
+  const int tiles_m = count_tiles<BM>(l);
+  int tile_m, tile_n, group, m0, m1;
+  if (!wide_tile(tiles_m, tiles_n, blockIdx.x, tile_m, tile_n) || !find_tile<BM>(l, tile_m, group, m0, m1)) return;
   const int n0 = tile_n * (GATED ? BN / 2 : BN);
   const char* a = l.a;
   const char* w = l.w + (int64_t)group * l.w_stride * ES;
