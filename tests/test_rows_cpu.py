@@ -213,3 +213,16 @@ int main() {
     assert r.returncode == 0, (r.returncode, r.stdout)
     # and the kernel counts no further
     assert "reduce<64>(min(tiles, most), [](int a, int b) { return a + b; }), most)" in open(os.path.join(csrc, "fc_groups.h")).read()
+
+
+def test_a_stream_of_another_device_is_refused(bz):
+    """a launch on it would run there, on memory that is here"""
+    class Stream:
+        device_index, cuda_stream = 1, 0
+
+    def bz_route_topk(desc, stream):
+        raise AssertionError("launched")
+
+    with pytest.raises(bz.BlazeHipError, match="bz_route_topk: the stream is of device 1, the current one is 0"):
+        bz._call(bz_route_topk, b"", Stream(), 0)
+    assert bz.lib().bz_route_topk.__name__ == "bz_route_topk"

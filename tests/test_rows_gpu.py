@@ -1222,3 +1222,17 @@ def test_rows_of_more_chunks_than_a_launch_has_threads_move_and_merge(bz):
         assert torch.equal(xs[to[t, 0].long()], x[t])
     del x, xs
     torch.cuda.empty_cache()
+
+
+def test_calls_on_a_stream_of_this_device(bz):
+    import torch
+    side = torch.cuda.Stream()
+    logits = _normal(0, (40, 8))
+    want = bz.route_topk(logits, 2)
+    side.wait_stream(torch.cuda.current_stream())
+    got = bz.route_topk(logits, 2, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    got = bz.route_topk(logits, 2, stream=torch.cuda.default_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0])

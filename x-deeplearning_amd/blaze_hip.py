@@ -792,6 +792,8 @@ def _empty(shape, dtype, like, stream):
 
 
 def _call(entry, desc, stream, here):
+    if stream is not None and stream.device_index != here:
+        raise BlazeHipError("%s: the stream is of device %d, the current one is %d" % (entry.__name__, stream.device_index, here))
     rc = entry(desc, _raw_stream(here) if stream is None else stream.cuda_stream)
     if rc != 0:
         check(rc)
