@@ -1020,8 +1020,8 @@ __global__ __launch_bounds__(256, TM * TN > 8 || (DT == BZ_F32 && TM * TN > 2) ?
   // 32x32x16 where the fp32 instructions take 512.  An operand is converted once for all four waves, on its way to LDS: it comes through
   // registers, two stages ahead, and a stage's pieces lie in one of two places as three matrices of 64 bytes a row, chunk c of row r at
   // position c ^ ((r >> 2) & 3).  Bound by the conversions and the instructions that feed the matrix cores: 8192 rows, 2048 -> 2048 475 us, 145
-  // TFLOP/s (730 with fp32 instructions, in the tile kernel); 2048 x 2 rows of 896 -> 512 through 8 experts 40.6 without what finds doubtful sums (44.7 with each wave converting
-  // the fragments that it read).
+  // TFLOP/s (730 with fp32 instructions, in the tile kernel); 2048 x 2 rows of 896 -> 512 through 8 experts 41.2 (44.7 with each wave converting
+  // the fragments that it read, and without what finds doubtful sums).
   // A sum that is not finite, or small enough that what a split drops of its operands may count in it, is doubtful (bz::fc::doubtful): the
   // tile is multiplied again with fp32 instructions then, and such sums are taken from there (the others stay, so that no row's result
   // depends on what is in another).  For that the largest operand of each row is kept on the way, a twelfth of the
@@ -1364,8 +1364,10 @@ inline int64_t wide_cost(int64_t tiles, const int (&part)[AT_ONCE]) {
 // Longer, aligned: the wide kernel, and 2-byte layers with the tile that fills the rounds of workgroups best.  Larger tiles take less time
 // a product, but a round that is begun costs a whole one (us by 256x256, 128x128, 64x128 and 64x64: bf16, one layer of 8192 rows, K 1024,
 // N 2048 44.2, 48.5, -, -; 8192 rows x 2 of 8 groups, 1024x1024 76.8, 60.3, -, -; 2048 rows x 2 38.6, 22.7, 26.6, 24.6; 1536 rows x 2 37.7,
-// 19.7, 18.2, 23.0; 256 rows x 2 32.2, 15.2, 12.7, 10.6; 512 rows x 8 of 64 groups, K 768, N 2048 68.3, 55.5, 47.7, 52.1).  fp32 layers, whose
-// multiplications take the time, keep to 64 rows and columns (2048 rows x 2 of 8 groups, 896 -> 512: 43.8 and with 64x128 49.6).
+// 19.7, 18.2, 23.0; 256 rows x 2 32.2, 15.2, 12.7, 10.6; 512 rows x 8 of 64 groups, K 768, N 2048 68.3, 55.5, 47.7, 52.1).  fp32 layers keep to 64
+// rows and columns, which is what few tiles want (us by 64x64, 64x128 and 128x64: 2048 rows x 2 of 8 groups, 896 -> 512 46.5, 51.7, 53.0; 4096 x 2
+// of 16, 512 -> 512 48.5, 52.2, 53.8; 1000 x 4 of 32, 256 -> 1024 31.0, 33.2, 35.3; 3000 x 2 of 4, 1024 -> 256 38.1, 37.7, 39.4), though long batches
+// would take less with 64x128 (8192 rows of one group, 2048 -> 2048 490, 444, 445; 8192 x 2 of 8, 1024 -> 1024 261, 243, 250).
 // What is not aligned: the tile kernel, which needs no alignment (where not the few rows' one: 1023x1023, 500 rows 11.6 by that and 16.7 by
 // tiles, fp32 700 rows 54.7 and 49.6, with adapters fp16 300 rows 24.7 and 24.2).
 template <int DT, bool GATED, bool ADAPTERS>
