@@ -1236,3 +1236,21 @@ def test_calls_on_a_stream_of_this_device(bz):
     got = bz.route_topk(logits, 2, stream=torch.cuda.default_stream())
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("m", [20, 900])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rank", [1, 16])
+def test_fc_adapters_lose_no_more_than_a_factors_rounding(bz, m, dtype, rank):
+    """A factor is two bf16s; its product with `up`, whose numbers two bf16s hold, loses nothing but what fp32 sums lose: four products a
+    term and the sums, (4 + 4) * rank steps of the terms."""
+    import torch
+    n = 700
+    a, down = _normal(0, (m, 1), 1.0, dtype), _normal(1, (1, rank, 1), 1.0, dtype)
+    up, w = _normal(2, (1, n, rank), 1.0, dtype), torch.zeros((n, 1), dtype=_t(dtype), device="cuda")
+    y = bz.fc_adapters(a, w, 1, down, up, torch.zeros(m, dtype=torch.int32, device="cuda"), out_dtype=bz.F32)
+    v = a.float() * down[0, :, 0].float()  # (exact: the product of two numbers of 11 bits or fewer)
+    hi = v.bfloat16()
+    factor = hi.double() + (v - hi.float()).bfloat16().double()
+    want, size = factor @ up[0].double().t(), factor.abs() @ up[0].double().abs().t()
+    _close(y, want, 8 * rank * EPS * size, "y")

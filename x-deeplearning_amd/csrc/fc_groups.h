@@ -216,6 +216,7 @@ struct LowStep {
         u_lo = bounded(u_lo);  // (an infinity less itself)
       }
       if (__builtin_expect(any_unbounded(hi), 0)) hi_some = bounded(hi);
+      In<BZ_BF16>::mma(lo, u_lo, d);  // (up to 2^-16 of the product, as much as a factor's own rounding)
       In<BZ_BF16>::mma(lo, u_some, d);
       In<BZ_BF16>::mma(hi_some, u_lo, d);
       In<BZ_BF16>::mma(hi, u_hi, d);
